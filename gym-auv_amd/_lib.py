@@ -16,7 +16,7 @@ ABI_VERSION = 3
 N_MODEL = 16
 
 # auv_dtype
-F64, F32, I32, U8, I64 = 0, 1, 2, 3, 4
+F64, F32, I32, U8, I64, BF16, F16 = 0, 1, 2, 3, 4, 5, 6
 
 # auv_buffer
 (BUF_STATE, BUF_ACTION, BUF_RANGES, BUF_HIT, BUF_PERCEPTION, BUF_NAVIGATION,
@@ -50,6 +50,11 @@ STATS_MAX_ENVS = 1048576
 CNN_SHALLOW, CNN_2DEEP, CNN_DEEP = 0, 1, 2
 CNN_FEATURES, CNN_RISK = 0, 1
 
+# sequence operators
+SEQ_FORWARD, SEQ_BACKWARD, SEQ_STEP = 0, 1, 2
+GATE_PLAIN, GATE_SILU, GATE_SIGMOID = 0, 1, 2
+NORM_MAX_CHANNELS = 8192
+
 # every symbol include/auvsim.h declares
 EXPORTS = (
     "auv_version", "auv_last_error", "auv_create", "auv_destroy", "auv_set_rays",
@@ -59,7 +64,8 @@ EXPORTS = (
     "auv_cnn_forward", "auv_cnn_last_error", "auv_format_rows", "auv_format_rows_device", "auv_dataset_rows",
     "auv_profile_read", "auv_attach_cnn", "auv_generate_scene", "auv_host_alloc", "auv_host_free",
     "auv_risk_rows", "auv_episode_stats", "auv_episode_stats_static", "auv_train_shallow", "auv_train_cnn", "auv_set_path",
-    "auv_launch_info",
+    "auv_launch_info", "auv_seq_last_error", "auv_causal_conv_workspace", "auv_causal_conv", "auv_selective_scan_segments",
+    "auv_selective_scan_workspace", "auv_selective_scan", "auv_residual_norm_workspace", "auv_residual_norm",
 )
 
 
@@ -83,6 +89,36 @@ class AuvSceneParams(C.Structure):
 class AuvTrainParams(C.Structure):
     _fields_ = [("optimizer", C.c_int32), ("reserved", C.c_int32), ("lr", C.c_double), ("beta1", C.c_double),
                 ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("momentum", C.c_double)]
+
+
+def _fields(text):
+    """Fields of an argument block, in order: names ending in * are pointers, in ! a double, the others 64-bit counts and strides."""
+    kinds = {"*": C.c_void_p, "!": C.c_double}
+    return [(f.rstrip("*!"), kinds.get(f[-1], C.c_int64)) for f in text.split()]
+
+
+class AuvConvArgs(C.Structure):
+    _fields_ = _fields("""
+        device dtype batch length channels width silu x* x_row x_token weight* bias* start* start_row start_token lengths*
+        state* new_state* y* y_row y_token d_y* d_y_row d_y_token d_new_state* d_x* d_x_row d_x_token d_weight* d_bias*
+        d_state* workspace* workspace_bytes""")
+
+
+class AuvScanArgs(C.Structure):
+    _fields_ = _fields("""
+        device dtype batch length channels states groups softplus u* u_row u_token delta* delta_row delta_token
+        z* z_row z_token B* B_row B_token B_group C* C_row C_token C_group A* D* delta_bias* start* start_row start_token
+        lengths* state* new_state* y* y_row y_token segments* d_y* d_y_row d_y_token d_new_state* d_u* d_u_row d_u_token
+        d_delta* d_delta_row d_delta_token d_z* d_z_row d_z_token d_B* d_B_row d_B_token d_B_group d_C* d_C_row d_C_token
+        d_C_group d_A* d_D* d_delta_bias* d_state* workspace* workspace_bytes""")
+
+
+class AuvNormArgs(C.Structure):
+    _fields_ = _fields("""
+        device dtype residual_dtype batch length channels gate_act eps! x* x_row x_token y* y_row y_token
+        gate* gate_row gate_token post_weight* pre_weight* scale* x_out* x_out_row x_out_token h* h_row h_token
+        d_x_out* d_x_out_row d_x_out_token d_h* d_h_row d_h_token d_x* d_x_row d_x_token d_y* d_y_row d_y_token
+        d_gate* d_gate_row d_gate_token d_post_weight* d_pre_weight* d_scale* workspace* workspace_bytes""")
 
 
 class AuvError(RuntimeError):
@@ -188,5 +224,15 @@ def load():
     lib.auv_train_cnn.argtypes = [i32] + lib.auv_train_shallow.argtypes
     lib.auv_set_path.restype = C.c_int
     lib.auv_set_path.argtypes = [vp, i32, i32, vp, i32, vp]
+    lib.auv_seq_last_error.restype = C.c_char_p
+    lib.auv_seq_last_error.argtypes = []
+    lib.auv_selective_scan_segments.restype = i64
+    lib.auv_selective_scan_segments.argtypes = [C.POINTER(AuvScanArgs)]
+    for name, args in (("auv_causal_conv", AuvConvArgs), ("auv_selective_scan", AuvScanArgs), ("auv_residual_norm", AuvNormArgs)):
+        call, room = getattr(lib, name), getattr(lib, name + "_workspace")
+        call.restype = C.c_int
+        call.argtypes = [C.POINTER(args), i32, vp]
+        room.restype = i64
+        room.argtypes = [C.POINTER(args), i32]
     _lib = lib
     return lib

@@ -111,15 +111,36 @@ class LidarCNN:
 
 class PerceptionNavigationExtractor:
     """What radarCNN.py:195-280 computes per policy step: the frozen CNN's
-    features of obs["perception"] concatenated with obs["navigation"][:,0,:]."""
+    features of obs["perception"] concatenated with obs["navigation"][:,0,:].
 
-    def __init__(self, kind: str, state_dict, device: int = 0):
+    With `memory`, a `memory.EpisodeMemory` over those features, each call is
+    one token of every env's episode and returns the memory's features instead;
+    `start` (B,) marks the envs whose episode begins with this observation
+    (`sim.tensor("t_step") == 0`).  The state of the batch is kept between
+    calls; `reset()` forgets it."""
+
+    def __init__(self, kind: str, state_dict, device: int = 0, memory=None):
         self.cnn = LidarCNN(kind, state_dict, device)
-        self.features_dim = self.cnn.out_dim("features") + 6
+        self.memory = memory
+        self._state = None
+        width = self.cnn.out_dim("features") + 6
+        if memory is not None and memory.features != width:
+            raise ValueError(f"the memory takes {memory.features} features, the extractor has {width}")
+        self.features_dim = width if memory is None else memory.channels
 
-    def __call__(self, obs):
+    def reset(self):
+        self._state = None
+
+    def __call__(self, obs, start=None):
         import torch
 
         per = self.cnn.forward(obs["perception"], "features")
         nav = obs["navigation"][:, 0, :]
-        return torch.cat([per, nav], dim=1)
+        out = torch.cat([per, nav], dim=1)
+        if self.memory is None:
+            if start is not None:
+                raise ValueError("start marks episodes for a memory; this extractor has none")
+            return out
+        if self._state is None:
+            self._state = self.memory.new_state(len(out))
+        return self.memory.step(out, self._state, start)

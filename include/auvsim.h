@@ -80,7 +80,8 @@ typedef struct auv_config {
                                (data/metadata_MovingObstaclesNoRules.csv rows 7362-7366, counting from 0) */
 } auv_config;
 
-typedef enum auv_dtype { AUV_F64 = 0, AUV_F32 = 1, AUV_I32 = 2, AUV_U8 = 3, AUV_I64 = 4 } auv_dtype;
+typedef enum auv_dtype { AUV_F64 = 0, AUV_F32 = 1, AUV_I32 = 2, AUV_U8 = 3, AUV_I64 = 4,
+                         AUV_BF16 = 5, AUV_F16 = 6 /* activations of the sequence operators only */ } auv_dtype;
 
 /* Device buffers a caller may borrow (shape in elements). */
 typedef enum auv_buffer {
@@ -461,6 +462,172 @@ int auv_train_cnn(int32_t kind, int device, const float* X, const float* y, int6
  * Synchronises the device.  Replaces the extractor's per-step CNN call,
  * radarCNN.py:270-280. */
 int auv_attach_cnn(auv_handle h, auv_cnn_handle c, int32_t head);
+
+/* ---- memory over an episode: sequence operators -----------------------------
+ * What a recurrent feature extractor is made of (a single scan shows no
+ * obstacle's velocity; the reference's loader stacks earlier scans for that,
+ * utils/dataloader.py:123-137): a short causal convolution, a selective state
+ * space scan, and the norms round a block.  Each works on whole rollouts
+ * [batch, length, channels] (rows = vessels, tokens = steps; any row and token
+ * strides, so a rollout stored time-major needs no copy), backwards for
+ * training, and the first two also on one token per row with the state kept
+ * between calls, for stepping.
+ *
+ * `dtype` is the type of all activations of a call (AUV_F32, AUV_BF16,
+ * AUV_F16); parameters, states of the scan, and their gradients are f32.  All
+ * arithmetic is in 32 bits, and every output is rounded once.  Strides count
+ * elements; channels are adjacent.  All pointers are DEVICE memory on
+ * `device`; what a call writes must not overlap what it reads, except where
+ * said.  `start` u8 (NULL: none): nonzero marks the first token of an
+ * episode; nothing before it is seen by it or by what follows.  `lengths`
+ * i32 [batch] (NULL: all): tokens a row really holds, clamped to [0, length];
+ * the tokens behind are not used, and their outputs and gradients are 0.
+ *
+ * Each call enqueues its kernels on `stream`, allocates nothing and never
+ * synchronises, so it may be captured into a graph; the scratch memory it
+ * needs is the caller's (`workspace`, at least auv_*_workspace(args, pass)
+ * bytes; calls that may overlap need one each).  The same inputs give the same
+ * bits on every call.  Errors: auv_seq_last_error(), of the calling thread.
+ */
+#define AUV_SEQ_FORWARD 0
+#define AUV_SEQ_BACKWARD 1
+#define AUV_SEQ_STEP 2
+const char* auv_seq_last_error(void);
+
+/* pre[b,l,d] = bias[d] + sum_j weight[d,j] x[b,l-(width-1)+j,d], y = pre or (silu) pre * sigmoid(pre).
+ * FORWARD: x, weight, bias, start, lengths, state -> y, new_state.
+ * BACKWARD: those (not new_state, y) and d_y, d_new_state (NULL: 0) -> d_x, d_weight, d_bias, d_state (NULL: not
+ *   wanted).
+ * STEP: length 1; x, state -> y, new_state, which may be state's own memory; `lengths` is not looked at. */
+typedef struct auv_conv_args {
+    int64_t device, dtype, batch, length, channels;
+    int64_t width;                /* 2, 3 or 4 taps */
+    int64_t silu;
+    const void* x;                /* [batch, length, channels] */
+    int64_t x_row, x_token;
+    const float* weight;          /* [channels, width], the last tap is the current token's */
+    const float* bias;            /* [channels] or NULL */
+    const uint8_t* start;         /* [batch, length] or NULL */
+    int64_t start_row, start_token;
+    const int32_t* lengths;       /* [batch] or NULL */
+    const void* state;            /* [batch, width-1, channels], the tokens before the row, oldest first; NULL: zeros */
+    void* new_state;              /* the same of the row's end, or NULL */
+    void* y;
+    int64_t y_row, y_token;
+    const void* d_y;
+    int64_t d_y_row, d_y_token;
+    const void* d_new_state;
+    void* d_x;
+    int64_t d_x_row, d_x_token;
+    float* d_weight;
+    float* d_bias;
+    void* d_state;
+    void* workspace;
+    int64_t workspace_bytes;
+} auv_conv_args;
+int64_t auv_causal_conv_workspace(const auv_conv_args* args, int32_t pass);   /* bytes, or a negative auv_status */
+int auv_causal_conv(const auv_conv_args* args, int32_t pass, void* stream);
+
+/* dt = softplus(delta + delta_bias) (or the sum itself); h[n] <- exp(dt A[d,n]) h[n] + dt u B[g,n];
+ * y = (sum_n C[g,n] h[n] + D[d] u) * z sigmoid(z)  (D, delta_bias, z: may be NULL); g = d / (channels / groups).
+ * FORWARD: ... -> y, new_state (or NULL), and, where a backward pass will follow, segments.
+ * BACKWARD: the same inputs, segments, d_y, d_new_state (NULL: 0) -> d_u, d_delta, d_A, d_B, d_C, d_D, d_z (with z),
+ *   d_delta_bias, d_state (the pointers to f32 gradients may be NULL: not wanted).
+ * STEP: length 1; state -> y, new_state, which may be state's own memory; `lengths` is not looked at. */
+typedef struct auv_scan_args {
+    int64_t device, dtype, batch, length, channels;
+    int64_t states;               /* 1 to 64 */
+    int64_t groups;               /* divides channels */
+    int64_t softplus;
+    const void* u;                /* [batch, length, channels] */
+    int64_t u_row, u_token;
+    const void* delta;
+    int64_t delta_row, delta_token;
+    const void* z;                /* or NULL */
+    int64_t z_row, z_token;
+    const void* B;                /* [batch, length, groups, states], states adjacent */
+    int64_t B_row, B_token, B_group;
+    const void* C;
+    int64_t C_row, C_token, C_group;
+    const float* A;               /* [channels, states] */
+    const float* D;               /* [channels] or NULL */
+    const float* delta_bias;      /* [channels] or NULL */
+    const uint8_t* start;
+    int64_t start_row, start_token;
+    const int32_t* lengths;
+    const float* state;           /* [batch, channels, states], before the row; NULL: zeros */
+    float* new_state;             /* behind it, or NULL */
+    void* y;
+    int64_t y_row, y_token;
+    float* segments;              /* auv_selective_scan_segments(args) bytes: states kept for the backward pass */
+    const void* d_y;
+    int64_t d_y_row, d_y_token;
+    const float* d_new_state;
+    void* d_u;
+    int64_t d_u_row, d_u_token;
+    void* d_delta;
+    int64_t d_delta_row, d_delta_token;
+    void* d_z;
+    int64_t d_z_row, d_z_token;
+    void* d_B;
+    int64_t d_B_row, d_B_token, d_B_group;
+    void* d_C;
+    int64_t d_C_row, d_C_token, d_C_group;
+    float* d_A;
+    float* d_D;
+    float* d_delta_bias;
+    float* d_state;
+    void* workspace;
+    int64_t workspace_bytes;
+} auv_scan_args;
+int64_t auv_selective_scan_segments(const auv_scan_args* args);
+int64_t auv_selective_scan_workspace(const auv_scan_args* args, int32_t pass);
+int auv_selective_scan(const auv_scan_args* args, int32_t pass, void* stream);
+
+/* n = y rsqrt(mean(y^2) + eps) post_weight (post_weight NULL: n = y); x_out = x + scale act(gate) n (scale, gate NULL:
+ * 1); h = x_out rsqrt(mean(x_out^2) + eps) pre_weight (pre_weight NULL: h is not formed; y NULL: h of x itself).
+ * x and x_out are of `residual_dtype` (AUV_F32 or dtype), y, gate and h of `dtype`.
+ * BACKWARD takes x (not x_out), y, gate, d_x_out (NULL: 0), d_h (NULL: 0) -> d_x, d_y, d_gate, and the f32 gradients
+ * (NULL: not wanted). */
+#define AUV_GATE_PLAIN 0
+#define AUV_GATE_SILU 1
+#define AUV_GATE_SIGMOID 2
+#define AUV_NORM_MAX_CHANNELS 8192
+typedef struct auv_norm_args {
+    int64_t device, dtype, residual_dtype, batch, length, channels;
+    int64_t gate_act;
+    double eps;
+    const void* x;
+    int64_t x_row, x_token;
+    const void* y;
+    int64_t y_row, y_token;
+    const void* gate;
+    int64_t gate_row, gate_token;
+    const float* post_weight;     /* [channels] or NULL */
+    const float* pre_weight;
+    const float* scale;
+    void* x_out;
+    int64_t x_out_row, x_out_token;
+    void* h;
+    int64_t h_row, h_token;
+    const void* d_x_out;
+    int64_t d_x_out_row, d_x_out_token;
+    const void* d_h;
+    int64_t d_h_row, d_h_token;
+    void* d_x;
+    int64_t d_x_row, d_x_token;
+    void* d_y;
+    int64_t d_y_row, d_y_token;
+    void* d_gate;
+    int64_t d_gate_row, d_gate_token;
+    float* d_post_weight;
+    float* d_pre_weight;
+    float* d_scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} auv_norm_args;
+int64_t auv_residual_norm_workspace(const auv_norm_args* args, int32_t pass);
+int auv_residual_norm(const auv_norm_args* args, int32_t pass, void* stream);
 
 #ifdef __cplusplus
 }
