@@ -42,7 +42,7 @@ constexpr int norm_threads() { return TPR < 256 ? 256 : TPR; }
 template <int TPR, int NSUM>
 __device__ __forceinline__ void row_sum(float (&v)[NSUM], float (*buf)[NSUM]) {
 #pragma unroll
-    for (int k = 0; k < NSUM; ++k) v[k] = lane_sum<0, (TPR >= 64 ? 6 : 4)>(v[k]);
+    for (int k = 0; k < NSUM; ++k) v[k] = lane_sum<(TPR >= 64 ? 6 : 4)>(v[k]);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         const int wave = threadIdx.x >> 6;

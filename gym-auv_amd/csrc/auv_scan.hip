@@ -51,7 +51,7 @@ struct Backward {
 };
 Backward backward_plan(const auv_scan_args& p) {
     const int S = lanes_of(p.states);
-    const int64_t waves = S <= 4 ? 8 : 4, tiles = tiles_of(p, S);
+    const int64_t waves = S <= 4 ? 8 : 4 /* scan_back_waves */, tiles = tiles_of(p, S);
     Backward r;
     r.per = tiles < waves ? tiles : waves;
     r.units = waves / r.per;
@@ -132,8 +132,8 @@ int run_forward(ScanArgs a, const Forward& f, hipStream_t stream) {
 
 template <class T, int S>
 int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStream_t stream) {
-    constexpr size_t lds = scan_back_lds<S>();
-    static_assert(lds <= 160 * 1024, "the tile's elements and sums must fit the CU's LDS");
+    static_assert(scan_back_lds<S>(scan_back_waves<S>()) <= 160 * 1024, "the tile's elements and sums must fit the CU's LDS");
+    const size_t lds = scan_back_lds<S>((int)r.units);
     constexpr int threads = scan_back_waves<S>() * 64;
     if (lds > 64 * 1024) {
         for (const void* k : {reinterpret_cast<const void*>(&k_scan_backward<T, S, 0>), reinterpret_cast<const void*>(&k_scan_backward<T, S, 1>)}) {
@@ -207,6 +207,13 @@ int by_states(const auv_scan_args& p, int32_t pass, ScanArgs a, hipStream_t stre
         }
     }
     const Backward r = backward_plan(p);
+    Width fours(4);
+    fours.stride(a.D / a.G);
+    for (const void* q : {a.u, a.delta, a.z, a.dy, (const void*)a.du, (const void*)a.ddelta, (const void*)a.dz}) fours.pointer(q, sizeof(T));
+    for (int64_t s : {a.u_row, a.u_token, a.delta_row, a.delta_token, a.z_row, a.z_token, a.dy_row, a.dy_token, a.du_row, a.du_token,
+                      a.ddelta_row, a.ddelta_token, a.dz_row, a.dz_token})
+        fours.stride(s);
+    a.whole = fours.elements() == 4;
     a.chunk = r.chunks.length, a.chunks = r.chunks.count;
     char* w = (char*)p.workspace;
     a.chunk_state = (float*)w;

@@ -12,6 +12,8 @@
 // multiplications and two fused multiply-adds on the vector unit.
 #pragma once
 
+#include <type_traits>
+
 #include "auv_seq.hpp"
 #include "auv_conv.hpp"   // row_length
 
@@ -49,6 +51,7 @@ struct ScanArgs {
     int64_t dB_row, dB_token, dB_group, dC_row, dC_token, dC_group;
     float* dstate;           // [B,D,N]
     float* partial;          // [gridDim.x * units per workgroup, D, N + 2]: dA, dD, ddelta_bias
+    int32_t whole;           // rows of activations and of their gradients may be read and written in fours
     float* bc_partial;       // [tile blocks, B, L, G, 2, NP] when a group's channels fill more than one workgroup
 };
 
@@ -71,12 +74,15 @@ __device__ __forceinline__ float step_slope(float raw, int softplus) { return so
 // MODE 1 starts each chunk from zero and leaves only its end state and its decay, exp(A sum dt) (0 behind a start).
 // ----------------------------------------------------------------------------------------------------------------
 constexpr int kScanTile = 8;
+template <int S>
+constexpr int lane_bits() { return S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0; }
 
 template <class T, int NPL, int S, int MODE>
 __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
-    constexpr int NP = NPL * S, CW = 64 / S, TQ = kScanTile;
+    constexpr int NP = NPL * S, CW = 64 / S, TQ = kScanTile, SB = lane_bits<S>();
+    constexpr int BE = (TQ * NP + 63) / 64;   // elements of B (and of C) a lane carries into LDS per tile
     __shared__ __align__(16) float tile[kScanWaves][TQ][2][NP];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int q = lane % S, c = lane / S;
     const int64_t Dg = a.D / a.G, tiles = (Dg + CW - 1) / CW;
     int64_t id = (int64_t)blockIdx.x * kScanWaves + wave;
@@ -86,8 +92,10 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
     id /= a.G;
     const int64_t b = id % a.B, chunk = id / a.B;
     if (chunk >= a.chunks) return;
-    const bool live = ct * CW + c < Dg;
-    const int64_t d = g * Dg + (live ? ct * CW + c : Dg - 1);
+    const int d_first = (int)(g * Dg + ct * CW), d_left = (int)(Dg - ct * CW);
+    const bool live = c < d_left;
+    const int dl = live ? c : d_left - 1;      // channel within the wave's tile
+    const int64_t d = d_first + dl;
     const int64_t n = row_length(a.lengths, b, a.L);
     const int64_t t_begin = chunk * a.chunk, t_end = t_begin + a.chunk < a.L ? t_begin + a.chunk : a.L;
     const int64_t stop = t_end < n ? t_end : n;
@@ -104,65 +112,101 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
         }
     }
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dv ? a.Dv[d] : 0.0f;
-    const T* const u = (const T*)a.u + b * a.u_row + d;
-    const T* const delta = (const T*)a.delta + b * a.delta_row + d;
-    const T* const z = (const T*)a.z + b * a.z_row + d;
+    // the wave's place in each array is a scalar; a lane adds its channel
+    const T* const u = (const T*)a.u + b * a.u_row + d_first;
+    const T* const delta = (const T*)a.delta + b * a.delta_row + d_first;
+    const T* const z = (const T*)a.z + b * a.z_row + d_first;
     const T* const Bm = (const T*)a.Bm + b * a.B_row + g * a.B_group;
     const T* const Cm = (const T*)a.Cm + b * a.C_row + g * a.C_group;
-    T* const y = (T*)a.y + b * a.y_row + d;
+    T* const y = (T*)a.y + b * a.y_row + d_first;
     float sum_dt = 0.0f;
     bool cut = false;
 
+    // what a tile needs from memory, fetched one tile ahead
+    T ru[TQ], rd[TQ], rz[TQ], rB[BE], rC[BE];
+    uint8_t mark = 0;
+    auto fetch = [&](int64_t t0) {
+        if (t0 >= stop) return;
+        const int left = stop - t0 < TQ ? (int)(stop - t0) : TQ;
+#pragma unroll
+        for (int i = 0; i < TQ; ++i) {
+            const int64_t t = t0 + (i < left ? i : left - 1);
+            ru[i] = (u + t * a.u_token)[dl];
+            rd[i] = (delta + t * a.delta_token)[dl];
+            if (MODE == 0 && a.z) rz[i] = (z + t * a.z_token)[dl];
+        }
+#pragma unroll
+        for (int k = 0; k < BE; ++k) {
+            const int e = k * 64 + lane, i = e / NP, s = e % NP;
+            const bool in = i < left && s < a.N;
+            rB[k] = in ? (Bm + t0 * a.B_token)[i * a.B_token + s] : (T)0.0f;
+            if (MODE == 0) rC[k] = in ? (Cm + t0 * a.C_token)[i * a.C_token + s] : (T)0.0f;
+        }
+        mark = 0;
+        if (a.start && lane < left) mark = a.start[b * a.start_row + (t0 + lane) * a.start_token];
+    };
+    fetch(t_begin);
     for (int64_t t0 = t_begin; t0 < stop; t0 += TQ) {
+        const int left = stop - t0 < TQ ? (int)(stop - t0) : TQ;
         if (MODE == 0 && a.segments && t0 % kSegment == 0 && live) {
             float* const seg = a.segments + ((b * ((a.L + kSegment - 1) / kSegment) + t0 / kSegment) * a.D + d) * NP + q * NPL;
 #pragma unroll
             for (int j = 0; j < NPL; j += 4) *reinterpret_cast<float4*>(seg + j) = make_float4(h[j], h[j + 1], h[j + 2], h[j + 3]);
         }
-        float uu[TQ], dd[TQ], zz[TQ];
+        const unsigned long long marks = __ballot(mark != 0);
+        float uu[TQ], dt[TQ], sz[TQ];
 #pragma unroll
         for (int i = 0; i < TQ; ++i) {
-            const int64_t t = t0 + i < stop ? t0 + i : stop - 1;
-            uu[i] = (float)u[t * a.u_token];
-            dd[i] = (float)delta[t * a.delta_token];
-            zz[i] = MODE == 0 && a.z ? (float)z[t * a.z_token] : 0.0f;
-        }
-        bool mark = false;
-        if (a.start && lane < TQ && t0 + lane < stop) mark = a.start[b * a.start_row + (t0 + lane) * a.start_token] != 0;
-        const unsigned long long marks = __ballot(mark);
-        wave_sync();
-#pragma unroll
-        for (int e0 = 0; e0 < TQ * NP; e0 += 64) {
-            const int e = e0 + lane, i = e / NP, s = e % NP;
-            if (TQ * NP >= 64 || e < TQ * NP) {
-                const bool in = t0 + i < stop && s < a.N;
-                tile[wave][i][0][s] = in ? (float)Bm[(t0 + i) * a.B_token + s] : 0.0f;
-                if (MODE == 0) tile[wave][i][1][s] = in ? (float)Cm[(t0 + i) * a.C_token + s] : 0.0f;
+            uu[i] = (float)ru[i];
+            dt[i] = step_width((float)rd[i] + bias, a.softplus);
+            sz[i] = 1.0f;
+            if (MODE == 0 && a.z) {
+                const float zz = (float)rz[i];
+                sz[i] = zz * sigmoid_f(zz);
             }
         }
         wave_sync();
 #pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            if (t0 + i < stop) {
-                if (marks >> i & 1) {
-                    cut = true;
+        for (int k = 0; k < BE; ++k) {
+            const int e = k * 64 + lane, i = e / NP, s = e % NP;
+            if (TQ * NP >= 64 || e < TQ * NP) {
+                tile[wave][i][0][s] = (float)rB[k];
+                if (MODE == 0) tile[wave][i][1][s] = (float)rC[k];
+            }
+        }
+        wave_sync();
+        fetch(t0 + TQ);
+        auto token = [&](int i) {
+            const float du = dt[i] * uu[i];
+            if (MODE == 1) sum_dt += dt[i];
+            float e[NPL], acc0 = 0.0f, acc1 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < NPL; ++j) h[j] = 0.0f;
-                }
-                const float dt = step_width(dd[i] + bias, a.softplus), du = dt * uu[i];
-                if (MODE == 1) sum_dt += dt;
-                float acc = 0.0f;
+            for (int j = 0; j < NPL; ++j) e[j] = exp2_hw(dt[i] * A2[j]);
 #pragma unroll
-                for (int j = 0; j < NPL; ++j) {
-                    const float e = exp2_hw(dt * A2[j]);
-                    h[j] = fmaf(e, h[j], du * tile[wave][i][0][q * NPL + j]);
-                    if (MODE == 0) acc = fmaf(h[j], tile[wave][i][1][q * NPL + j], acc);
+            for (int j = 0; j < NPL; ++j) h[j] = fmaf(e[j], h[j], du * tile[wave][i][0][q * NPL + j]);
+            if (MODE == 0) {
+#pragma unroll
+                for (int j = 0; j < NPL; j += 2) {
+                    acc0 = fmaf(h[j], tile[wave][i][1][q * NPL + j], acc0);
+                    acc1 = fmaf(h[j + 1], tile[wave][i][1][q * NPL + j + 1], acc1);
                 }
-                if (MODE == 0) {
-                    acc = lane_sum<0, (S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0)>(acc);
-                    acc = fmaf(skip, uu[i], acc);
-                    if (a.z) acc *= zz[i] * sigmoid_f(zz[i]);
-                    if (live && q == 0) y[(t0 + i) * a.y_token] = (T)acc;
+                const float sum = lane_sum<SB>(acc0 + acc1);
+                if (live && q == 0) (y + (t0 + i) * a.y_token)[dl] = (T)(fmaf(skip, uu[i], sum) * sz[i]);
+            }
+        };
+        if (left == TQ && marks == 0) {
+#pragma unroll
+            for (int i = 0; i < TQ; ++i) token(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TQ; ++i) {
+                if (i < left) {
+                    if (marks >> i & 1) {
+                        cut = true;
+#pragma unroll
+                        for (int j = 0; j < NPL; ++j) h[j] = 0.0f;
+                    }
+                    token(i);
                 }
             }
         }
@@ -184,7 +228,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
             if (q * NPL + j < a.N) a.new_state[(b * a.D + d) * a.N + q * NPL + j] = h[j];
     }
     if (live && q == 0)
-        for (int64_t t = t_begin > n ? t_begin : n; t < t_end; ++t) y[t * a.y_token] = (T)0.0f;
+        for (int64_t t = t_begin > n ? t_begin : n; t < t_end; ++t) (y + t * a.y_token)[dl] = (T)0.0f;
 }
 
 // Joins the chunks of a row: chunk_state[c] becomes the state the chunk starts from (forwards from `state`) or, going
@@ -246,258 +290,445 @@ __global__ __launch_bounds__(64 * kJoinRows) void k_scan_join(JoinArgs a) {
 // channels: over the lanes of a wave, then over the waves of the workgroup through LDS, in a fixed order.  dA, dD and
 // ddelta_bias are sums over rows and tokens: each wave keeps them in registers over all rows it works on.
 // ----------------------------------------------------------------------------------------------------------------
+// The element-wise parts (widths, gates and their derivatives; the stores of du, ddelta, dz) belong to the workgroup: a
+// thread takes four adjacent channels of a token, so that loads and stores are 8 or 16 bytes wide and a token's channels
+// go in one piece.  Two-byte accesses by the lanes of the sweeps, 32 bytes of a token at a time, took longer than the
+// arithmetic.
 template <int S>
 constexpr int scan_back_waves() { return S <= 4 ? 8 : 4; }
+// tokens whose states a lane holds at a time: half a segment, so that two waves more fit on a SIMD (with S = 16 the sums
+// over a channel's lanes want all sixteen together)
 template <int S>
-constexpr size_t scan_back_lds() {
-    constexpr int NP = 4 * S, CW = 64 / S, W = scan_back_waves<S>();
-    // per wave: dt, u, g, - of 16 tokens x CW channels; B and C of 16 tokens; sums of 16 tokens
-    return (size_t)W * 4 * (16 * CW * 4 + 16 * 2 * NP + 16 * 2 * NP);
+constexpr int scan_back_hold() { return S <= 8 ? 8 : 16; }
+template <int S>
+constexpr size_t scan_back_lds(int units) {
+    constexpr int NP = 4 * S, W = scan_back_waves<S>(), CH = 64 / S * W;
+    // per token and channel four numbers; delta_bias and D per channel; sums of dD and ddelta_bias per thread; sums of dB
+    // and dC per wave; row lengths; B and C per row
+    return (size_t)4 * (4 * 16 * CH + 2 * CH + 2 * 4 * W * 64 + W * 16 * 2 * NP + 2 * W + units * 16 * 2 * NP);
+}
+
+// The kernel's arguments, read where they are used: some sixty addresses and strides held in scalar registers through
+// the tile loop would push its own scalars out to vector lanes.
+__device__ __forceinline__ ScanArgs scan_args() {
+    const __attribute__((address_space(4))) ScanArgs* p = (const __attribute__((address_space(4))) ScanArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    ScanArgs r;
+    __builtin_memcpy(&r, (const ScanArgs*)p, sizeof(ScanArgs));
+    return r;
+}
+
+// Four adjacent channels of one token as they lie in memory, in 32-bit words: taking the elements out, or merging them
+// with the zeros of a load left out, would wait for the load there and then.
+template <class T>
+struct Quad {
+    unsigned w[sizeof(T)];
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[j]);
+        else return (float)__builtin_bit_cast(T, (unsigned short)(w[j / 2] >> (16 * (j % 2))));
+    }
+};
+// `count` of the four are real (the others come out as 0); `whole`: the address allows one access.
+template <class T>
+__device__ __forceinline__ void load4(Quad<T>& out, const T* p, int count, bool whole) {
+    using Words = Vec<unsigned, sizeof(T)>;
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T); ++j) out.w[j] = 0;
+    if (whole) {
+        if (count == 4) {
+            const Words t = *reinterpret_cast<const Words*>(p);
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T); ++j) out.w[j] = t.v[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) {
+                if constexpr (sizeof(T) == 4) out.w[j] = reinterpret_cast<const unsigned*>(p)[j];
+                else out.w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
+            }
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, int count, bool whole, const float (&in)[4]) {
+    if (whole) {
+        if (count == 4) store<T, 4>(p, in);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) p[j] = (T)in[j];
+    }
+}
+
+// The thread's number, in a form whose derivatives the compiler does not carry from one use to the next.
+__device__ __forceinline__ int thread_anew() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
 }
 
 // MODE 0: gradients.  MODE 1: from zero at the end of each chunk, only the carry at its front and its decay.
 template <class T, int S, int MODE>
-__global__ __launch_bounds__(scan_back_waves<S>() * 64) void k_scan_backward(ScanArgs a) {
-    constexpr int NP = 4 * S, CW = 64 / S, W = scan_back_waves<S>(), Q = kSegment, KT = Q / S;
-    constexpr int SB = S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0;
-    static_assert(S <= Q, "every lane of a channel has a token of its own to finish");
+__global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 : 2) void k_scan_backward(ScanArgs a) {
+    constexpr int NP = 4 * S, CW = 64 / S, W = scan_back_waves<S>(), Q = kSegment, HQ = scan_back_hold<S>(), KT = HQ / S, SB = lane_bits<S>();
+    constexpr int TH = W * 64, CH = W * CW;
+    constexpr int QUADS = CH / 4, STEP = TH / QUADS, IT = Q > STEP ? Q / STEP : 1;   // a thread's tokens: first, first + STEP, ...
+    constexpr int BE = Q * 2 * NP / 64;                                             // its share of B and C at the most
+    // dB and dC of GT tokens are summed over the wave's channels together: as many values as lanes to sum over
+    constexpr int GT = CW >= 8 ? CW / 8 : 1, GV = GT * 8, GR = GV / CW > 1 ? GV / CW : 1;
+    static_assert(S <= HQ && GT <= HQ && CW >= 4, "the sums over lanes are formed for whole groups of tokens");
     extern __shared__ __align__(16) float lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int q = lane % S, c = lane / S;
-    float(*const elem)[CW][4] = reinterpret_cast<float(*)[CW][4]>(lds + (size_t)wave * Q * CW * 4);
-    float(*const bc)[2][NP] = reinterpret_cast<float(*)[2][NP]>(lds + (size_t)W * Q * CW * 4 + (size_t)wave * Q * 2 * NP);
-    float* const red = lds + (size_t)W * (Q * CW * 4 + Q * 2 * NP);   // [wave][token][2][NP]
+    // [token][channel]: the step's width; width u, then the sweeps' s1; g, then the sum of through A2; the sum of C h
+    float(*const width)[CH] = reinterpret_cast<float(*)[CH]>(lds);
+    float(*const wu)[CH] = width + Q, (*const gate)[CH] = wu + Q, (*const sum_y)[CH] = gate + Q;
+    float(*const param)[CH] = sum_y + Q;                                                    // delta_bias, D
+    float(*const sums)[4] = reinterpret_cast<float(*)[4]>(param + 2);                       // a thread's dD, ddelta_bias
+    float* const red = lds + 4 * Q * CH + 2 * CH + 2 * 4 * TH;                              // [wave][token][2][NP]
+    int64_t* const len = reinterpret_cast<int64_t*>(red + W * Q * 2 * NP);                  // tokens of each row at work
+    float(*const bc_all)[Q][2][NP] = reinterpret_cast<float(*)[Q][2][NP]>(len + W);         // [row at work]
 
-    const int64_t Dg = a.D / a.G;
-    const int tiles = (int)((Dg + CW - 1) / CW);             // waves a group's channels take
+    const int Dg = (int)(a.D / a.G);
+    const int tiles = (Dg + CW - 1) / CW;                    // waves a group's channels take
     const int per = tiles < W ? tiles : W, units = W / per;  // ... of them in this workgroup; rows side by side in it
     const int blocks = (tiles + per - 1) / per;
-    const int unit = wave / per, ct = (int)(blockIdx.y % blocks) * per + wave % per;
-    const int64_t g = blockIdx.y / blocks;
     const int tb = blockIdx.y % blocks;
-    const bool working = unit < units;
-    const bool live = working && ct * CW + c < Dg;
-    const int64_t d = g * Dg + (live ? ct * CW + c : Dg - 1);
+    const int g = blockIdx.y / blocks;
+    const int N = a.N, softplus = a.softplus;
+    const bool gated = a.z != nullptr, whole = a.whole != 0;
 
-    float A[4], A2[4], dA[4];
+    // the sweeps' view: a lane has states 4 q .. 4 q + 3 of channel c of its wave
+    const int unit = wave / per, ct = tb * per + wave % per;
+    const bool working = unit < units && ct * CW < Dg;
+    const bool live = working && c < Dg - ct * CW;
+    const int64_t d = working ? g * Dg + ct * CW + (live ? c : Dg - ct * CW - 1) : 0;
+    float(*const bc)[2][NP] = bc_all[unit < units ? unit : 0];
+    float A2[4], dA[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int s = q * 4 + j;
-        A[j] = s < a.N ? a.A[d * a.N + s] : 0.0f;
-        A2[j] = A[j] * kLog2e;
+        A2[j] = s < N ? a.A[d * N + s] * kLog2e : 0.0f;
         dA[j] = 0.0f;
     }
-    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dv ? a.Dv[d] : 0.0f;
-    float dD = 0.0f, dbias = 0.0f;
-
-    const int64_t groups = (a.B + units - 1) / units;
-    for (int64_t item = blockIdx.x; item < groups * a.chunks; item += gridDim.x) {
-        const int64_t chunk = item / groups;
-        const int64_t row = (item % groups) * units + unit;
-        const bool on = working && row < a.B;                  // the same for all lanes of a wave
-        const int64_t b = row < a.B ? row : a.B - 1;
-        const int64_t n = on ? row_length(a.lengths, b, a.L) : 0;
-        const int64_t t_begin = chunk * a.chunk, t_end = t_begin + a.chunk < a.L ? t_begin + a.chunk : a.L;
-        const T* const u = (const T*)a.u + b * a.u_row + d;
-        const T* const delta = (const T*)a.delta + b * a.delta_row + d;
-        const T* const z = (const T*)a.z + b * a.z_row + d;
-        const T* const dy = (const T*)a.dy + b * a.dy_row + d;
-        const T* const Bm = (const T*)a.Bm + b * a.B_row + g * a.B_group;
-        const T* const Cm = (const T*)a.Cm + b * a.C_row + g * a.C_group;
-        float carry[4];
-        float sum_dt = 0.0f;
-        bool cut = false;
+    // the element-wise view: a thread has channels quad_d .. quad_d + quad_n - 1 of tokens quad_t, quad_t + STEP, ...
+    const int slot = threadIdx.x % QUADS * 4, quad_t = threadIdx.x / QUADS;
+    const int wave_t = uniform(wave * 64 / QUADS), lane_t = QUADS < 64 ? lane / QUADS : 0;    // quad_t = wave_t + lane_t
+    const int quad_unit = slot / CW / per, quad_c = (tb * per + slot / CW % per) * CW + slot % CW;
+    const int quad_n = quad_unit >= units || quad_t >= Q ? 0 : Dg - quad_c < 4 ? (Dg - quad_c > 0 ? Dg - quad_c : 0) : 4;
+    const int64_t quad_d = (int64_t)g * Dg + quad_c;
+    // where a thread's first token lies, from its workgroup's first row and its wave's first token: formed anew for each
+    // tile, the registers are worth more than the arithmetic
+    auto away = [&](int64_t row, int64_t token) {
+        int64_t at = quad_c;
+        if constexpr (QUADS == 32) at += lane_t ? token : 0;
+        else if constexpr (QUADS < 32) at += (int64_t)lane_t * token;
+        if (units > 1) at += (int64_t)quad_unit * row;
+        return at;
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[threadIdx.x][j] = sums[TH + threadIdx.x][j] = 0.0f;
+    if (quad_t == 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int s = q * 4 + j;
-            carry[j] = 0.0f;
-            if (MODE == 0 && on) {
-                if (a.chunks > 1) carry[j] = a.chunk_state[((chunk * a.B + b) * a.D + d) * NP + s];
-                else if (a.dnew_state && s < a.N) carry[j] = a.dnew_state[(b * a.D + d) * a.N + s];
+            param[0][slot + j] = a.bias && j < quad_n ? a.bias[quad_d + j] : 0.0f;
+            param[1][slot + j] = a.Dv && j < quad_n ? a.Dv[quad_d + j] : 0.0f;
+        }
+    }
+
+    const int64_t groups = (a.B + units - 1) / units, items = groups * a.chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t chunk = item / groups;
+        const int64_t row0 = (item - chunk * groups) * units;
+        int64_t b, n, t_begin, t_end;
+        bool on;
+        float carry[4];
+        {
+            const ScanArgs r = scan_args();
+            __syncthreads();
+            if ((int)threadIdx.x < units) len[threadIdx.x] = row0 + threadIdx.x < r.B ? row_length(r.lengths, row0 + threadIdx.x, r.L) : 0;
+            __syncthreads();
+            on = working && row0 + unit < r.B;                  // the same for all lanes of a wave
+            b = on ? row0 + unit : r.B - 1;
+            n = on ? row_length(r.lengths, b, r.L) : 0;
+            t_begin = chunk * r.chunk, t_end = t_begin + r.chunk < r.L ? t_begin + r.chunk : r.L;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int s = q * 4 + j;
+                carry[j] = 0.0f;
+                if (MODE == 0 && on) {
+                    if (r.chunks > 1) carry[j] = r.chunk_state[((chunk * r.B + b) * r.D + d) * NP + s];
+                    else if (r.dnew_state && s < N) carry[j] = r.dnew_state[(b * r.D + d) * N + s];
+                }
             }
         }
-        for (int64_t t0 = (t_end - 1) / Q * Q; t0 >= t_begin; t0 -= Q) {
-            const int here = t0 >= n ? 0 : n - t0 < Q ? (int)(n - t0) : Q;   // tokens of this row in the tile
-            bool mark = false;
-            if (a.start && lane < here) mark = a.start[b * a.start_row + (t0 + lane) * a.start_token] != 0;
-            const unsigned long long marks = __ballot(mark);
-            // element-wise part: lane q of a channel takes every S-th token
-            float out[KT], zz[KT], slope[KT], uu[KT], gg[KT];
-            wave_sync();
+        float sum_dt = 0.0f;
+        bool cut = false;
+
+        // what a tile needs from memory; the next tile's is asked for before this one's results are written
+        Quad<T> fu[IT] = {}, fd[IT] = {}, fz[IT] = {}, fy[IT] = {};
+        T fbc[BE] = {};
+        float4 fh = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        uint8_t mark = 0;
+        auto fetch = [&](int64_t t0) {
+            const ScanArgs r = scan_args();
+            const int64_t quad_len = quad_n > 0 ? len[quad_unit] : 0, quad_0 = t0 + wave_t;
+            auto from = [&](Quad<T>(&to)[IT], const void* base, int64_t row, int64_t token) {
+                const T* const p = (const T*)base + row0 * row + quad_0 * token + (int64_t)g * Dg;
+                const int64_t off = away(row, token);
 #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                const int i = k * S + q;
-                const int64_t t = i < here ? t0 + i : n > 0 ? n - 1 : 0;
-                const float raw = (float)delta[t * a.delta_token] + bias;
-                const float dt = step_width(raw, a.softplus);
-                out[k] = (float)dy[t * a.dy_token];
-                zz[k] = a.z ? (float)z[t * a.z_token] : 0.0f;
-                slope[k] = step_slope(raw, a.softplus);
-                uu[k] = MODE == 0 ? (float)u[t * a.u_token] : 0.0f;
-                gg[k] = a.z ? out[k] * (zz[k] * sigmoid_f(zz[k])) : out[k];
-                *reinterpret_cast<float4*>(&elem[i][c][0]) = make_float4(dt, uu[k], gg[k], dt * uu[k]);
+                for (int k = 0; k < IT; ++k)
+                    load4(to[k], p + k * STEP * token + off, quad_0 + k * STEP + lane_t < quad_len ? quad_n : 0, whole);
+            };
+            from(fd, r.delta, r.delta_row, r.delta_token);
+            from(fy, r.dy, r.dy_row, r.dy_token);
+            if (gated) from(fz, r.z, r.z_row, r.z_token);
+            if (MODE == 0) from(fu, r.u, r.u_row, r.u_token);
+            const int tid = thread_anew();
+#pragma unroll
+            for (int k = 0; k < BE; ++k) {
+                const int e = tid + k * TH;
+                if (k * TH < units * Q * 2 * NP) {
+                    const int un = e / (Q * 2 * NP), i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
+                    fbc[k] = (T)0.0f;
+                    if (un < units && s < N && t0 + i < len[un]) {
+                        const int64_t br = row0 + un;
+                        if (which == 1) fbc[k] = ((const T*)r.Cm + br * r.C_row + g * r.C_group + t0 * r.C_token)[i * r.C_token + s];
+                        else if (MODE == 0) fbc[k] = ((const T*)r.Bm + br * r.B_row + g * r.B_group + t0 * r.B_token)[i * r.B_token + s];
+                    }
+                }
             }
-            for (int e = lane; e < Q * NP; e += 64) {
-                const int i = e / NP, s = e % NP;
-                const bool in = i < here && s < a.N;
-                bc[i][0][s] = in && MODE == 0 ? (float)Bm[(t0 + i) * a.B_token + s] : 0.0f;
-                bc[i][1][s] = in ? (float)Cm[(t0 + i) * a.C_token + s] : 0.0f;
+            mark = 0;
+            if (r.start && lane < Q && t0 + lane < n) mark = r.start[b * r.start_row + (t0 + lane) * r.start_token];
+            if (MODE == 0 && t0 < n)
+                fh = *reinterpret_cast<const float4*>(r.segments + ((b * ((r.L + Q - 1) / Q) + t0 / Q) * r.D + d) * NP + q * 4);
+        };
+        const int64_t t_last = (t_end - 1) / Q * Q;
+        fetch(t_last);
+        for (int64_t t0 = t_last; t0 >= t_begin; t0 -= Q) {
+            const int here = t0 >= n ? 0 : n - t0 < Q ? (int)(n - t0) : Q;   // tokens of this wave's row in the tile
+            const unsigned marks = (unsigned)__ballot(mark != 0);
+            const float h0[4] = {fh.x, fh.y, fh.z, fh.w};
+            Quad<T> gu[IT], gd[IT], gz[IT], gy[IT];      // this tile's elements
+            const int64_t quad_len = quad_n > 0 ? len[quad_unit] : 0;
+            // param and, from the tile before, the elements, bc and red: everything is read by now
+            __syncthreads();
+            const int tid = thread_anew();
+#pragma unroll
+            for (int k = 0; k < BE; ++k) {
+                const int e = tid + k * TH;
+                if (e < units * Q * 2 * NP) (&bc_all[0][0][0][0])[e] = (float)fbc[k];
             }
-            wave_sync();
-            float s1[KT], s2[KT], yy[KT];
+#pragma unroll
+            for (int k = 0; k < IT; ++k) {
+                const int i = quad_t + k * STEP;
+                const int count = t0 + i < quad_len ? quad_n : 0;
+                gu[k] = fu[k], gd[k] = fd[k], gz[k] = fz[k], gy[k] = fy[k];
+                float w[4], x[4], o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // tokens behind the row's last and lanes without a channel: width 0 (decay 1), and they add nothing
+                    w[j] = j < count ? step_width(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
+                    x[j] = w[j] * gu[k].at(j);
+                    const float zz = gz[k].at(j);
+                    o[j] = gated ? gy[k].at(j) * (zz * sigmoid_f(zz)) : gy[k].at(j);
+                }
+                if (i < Q) {
+                    store<float, 4>(&width[i][slot], w);
+                    if (MODE == 0) store<float, 4>(&wu[i][slot], x);
+                    store<float, 4>(&gate[i][slot], o);
+                }
+            }
+            __syncthreads();
+            const int me = wave * CW + c, mine = lane_place<SB, 0, S>(lane);
             if (MODE == 1) {
+                if (t0 > t_begin) fetch(t0 - Q);
 #pragma unroll
                 for (int i = Q - 1; i >= 0; --i) {
-                    if (i < here) {
-                        const float4 el = *reinterpret_cast<const float4*>(&elem[i][c][0]);
-                        sum_dt += el.x;
+                    const float w = width[i][me], o = gate[i][me];
+                    sum_dt += w;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            carry[j] = fmaf(el.z, bc[i][1][q * 4 + j], carry[j]) * exp2_hw(el.x * A2[j]);
-                        if (marks >> i & 1) {
-                            cut = true;
+                    for (int j = 0; j < 4; ++j) carry[j] = fmaf(o, bc[i][1][q * 4 + j], carry[j]) * exp2_hw(w * A2[j]);
+                    if (marks >> i & 1) {
+                        cut = true;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) carry[j] = 0.0f;
-                        }
+                        for (int j = 0; j < 4; ++j) carry[j] = 0.0f;
                     }
                 }
                 continue;
             }
-            // the states of the tile's tokens, from the one kept before it
-            float hist[Q + 1][4];
-            if (here > 0) {
-                const float4 h0 = *reinterpret_cast<const float4*>(
-                    a.segments + ((b * ((a.L + Q - 1) / Q) + t0 / Q) * a.D + d) * NP + q * 4);
-                hist[0][0] = h0.x, hist[0][1] = h0.y, hist[0][2] = h0.z, hist[0][3] = h0.w;
-            } else {
+            // HQ tokens from `first` on, forwards and backwards.  STARTS: some token of the tile opens an episode.
+            auto sweep = [&](auto starts, int first) {
+                constexpr bool STARTS = decltype(starts)::value;
+                float hist[HQ + 1][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) hist[0][j] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                if (i < here) {
-                    const float4 el = *reinterpret_cast<const float4*>(&elem[i][c][0]);
-                    const bool fresh = marks >> i & 1;
-                    float acc = 0.0f;
+                for (int j = 0; j < 4; ++j) hist[0][j] = h0[j];
+                for (int i = 0; i < first; ++i) {       // up to the first of them, from the state kept before the tile
+                    const float w = width[i][me], x = wu[i][me];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float before = fresh ? 0.0f : hist[i][j];
-                        hist[i + 1][j] = fmaf(exp2_hw(el.x * A2[j]), before, el.w * bc[i][0][q * 4 + j]);
-                        acc = fmaf(hist[i + 1][j], bc[i][1][q * 4 + j], acc);
+                        float before = hist[0][j];
+                        if (STARTS && (marks >> i & 1)) before = 0.0f;
+                        hist[0][j] = fmaf(exp2_hw(w * A2[j]), before, x * bc[i][0][q * 4 + j]);
                     }
-                    acc = lane_sum<0, SB>(acc);
-                    if (i % S == q) yy[i / S] = acc;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) hist[i + 1][j] = hist[i][j];
-                    if (i % S == q) yy[i / S] = 0.0f;
                 }
-            }
-#pragma unroll
-            for (int i = Q - 1; i >= 0; --i) {
-                float db[4], dc[4];
-                float p1 = 0.0f, p2 = 0.0f;
-                if (i < here) {
-                    const float4 el = *reinterpret_cast<const float4*>(&elem[i][c][0]);
-                    const bool fresh = marks >> i & 1;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float dh = fmaf(el.z, bc[i][1][q * 4 + j], carry[j]);
-                        dc[j] = el.z * hist[i + 1][j];
-                        db[j] = dh * el.w;
-                        p1 = fmaf(dh, bc[i][0][q * 4 + j], p1);
-                        carry[j] = fresh ? 0.0f : dh * exp2_hw(el.x * A2[j]);
-                        const float through = fresh ? 0.0f : carry[j] * hist[i][j];
-                        p2 = fmaf(through, A[j], p2);
-                        dA[j] = fmaf(through, el.x, dA[j]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) db[j] = dc[j] = 0.0f;
-                }
-                p1 = lane_sum<0, SB>(p1);
-                p2 = lane_sum<0, SB>(p2);
-                if (i % S == q) s1[i / S] = p1, s2[i / S] = p2;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    db[j] = lane_sum<SB, 6>(live ? db[j] : 0.0f);
-                    dc[j] = lane_sum<SB, 6>(live ? dc[j] : 0.0f);
-                }
-                if (c == 0) {
-                    float* const to = red + ((size_t)(wave * Q + i) * 2) * NP + q * 4;
-                    *reinterpret_cast<float4*>(to) = make_float4(db[0], db[1], db[2], db[3]);
-                    *reinterpret_cast<float4*>(to + NP) = make_float4(dc[0], dc[1], dc[2], dc[3]);
-                }
-            }
-            if (live && on) {
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    const int i = k * S + q;
-                    const int64_t t = t0 + i;
-                    if (t < t_end) {
-                        const bool in = i < here;
-                        const float dt = elem[i][c][0];
-                        const float draw = in ? fmaf(s1[k], uu[k], s2[k]) * slope[k] : 0.0f;
-                        const float gu = in ? fmaf(s1[k], dt, gg[k] * skip) : 0.0f;
-                        ((T*)a.du + b * a.du_row + d)[t * a.du_token] = (T)gu;
-                        ((T*)a.ddelta + b * a.ddelta_row + d)[t * a.ddelta_token] = (T)draw;
-                        if (a.z) {
-                            const float sg = sigmoid_f(zz[k]);
-                            const float gz = in ? out[k] * fmaf(skip, uu[k], yy[k]) * (sg * fmaf(zz[k], 1.0f - sg, 1.0f)) : 0.0f;
-                            ((T*)a.dz + b * a.dz_row + d)[t * a.dz_token] = (T)gz;
+                    float part[S];
+#pragma unroll
+                    for (int o = 0; o < S; ++o) {
+                        const int m = k * S + o, i = first + m;
+                        const float w = width[i][me], x = wu[i][me];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float before = hist[m][j];
+                            if (STARTS && (marks >> i & 1)) before = 0.0f;
+                            hist[m + 1][j] = fmaf(exp2_hw(w * A2[j]), before, x * bc[i][0][q * 4 + j]);
+                            const float C = bc[i][1][q * 4 + j];
+                            part[o] = j == 0 ? hist[m + 1][j] * C : fmaf(hist[m + 1][j], C, part[o]);
                         }
-                        dbias += draw;
-                        if (in) dD = fmaf(gg[k], uu[k], dD);
+                    }
+                    lane_scatter_sum<SB, 0, S>(part);      // a channel's lanes get the sums of S tokens, one each
+                    sum_y[first + k * S + mine][me] = part[0];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float p1[S], p2[S], bcsum[GV], s1[KT], s2[KT];
+#pragma unroll
+                for (int m = HQ - 1; m >= 0; --m) {
+                    const int i = first + m;
+                    const float w = width[i][me], x = wu[i][me], o = gate[i][me];
+                    float x1, x2;
+                    float* const to = bcsum + (m % GT) * 8;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float dh = fmaf(o, bc[i][1][q * 4 + j], carry[j]);
+                        to[j] = dh * x;
+                        to[4 + j] = o * hist[m + 1][j];
+                        const float B = bc[i][0][q * 4 + j];
+                        x1 = j == 0 ? dh * B : fmaf(dh, B, x1);
+                        carry[j] = dh * exp2_hw(w * A2[j]);
+                        if (STARTS && (marks >> i & 1)) carry[j] = 0.0f;
+                        const float through = carry[j] * hist[m][j];
+                        x2 = j == 0 ? through * A2[j] : fmaf(through, A2[j], x2);
+                        dA[j] = fmaf(through, w, dA[j]);
+                    }
+                    p1[m % S] = x1, p2[m % S] = x2;
+                    if (m % S == 0) {
+                        lane_scatter_sum<SB, 0, S>(p1);
+                        lane_scatter_sum<SB, 0, S>(p2);
+                        s1[m / S] = p1[0], s2[m / S] = p2[0];
+                    }
+                    if (m % GT == 0) {
+                        lane_scatter_sum<6, SB, GV>(bcsum);
+                        // value v of GV is token i + v / 8, dB (0) or dC (1), state 4 q + v % 4
+                        const int v = lane_place<6, SB, GV>(lane);
+                        float* const at = red + ((wave * Q + i + v / 8) * 2 + v / 4 % 2) * NP + q * 4 + v % 4;
+#pragma unroll
+                        for (int r = 0; r < GR; ++r) at[r] = bcsum[r];
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-            }
-            __syncthreads();
-            for (int e = threadIdx.x; e < units * Q * 2 * NP; e += W * 64) {
-                const int un = e / (Q * 2 * NP), i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
-                const int64_t br = (item % groups) * units + un, t = t0 + i;
-                if (br < a.B && t < t_end && s < a.N) {
-                    float sum = 0.0f;
-                    for (int w = 0; w < per; ++w) sum += red[((size_t)((un * per + w) * Q + i) * 2 + which) * NP + s];
-                    if (a.bc_partial)
-                        a.bc_partial[((((int64_t)tb * a.B + br) * a.L + t) * a.G + g) * 2 * NP + which * NP + s] = sum;
-                    else if (which == 0)
-                        ((T*)a.dB + br * a.dB_row + t * a.dB_token + g * a.dB_group)[s] = (T)sum;
-                    else
-                        ((T*)a.dC + br * a.dC_row + t * a.dC_token + g * a.dC_group)[s] = (T)sum;
+                // these tokens' width u and g have been read for the last time, and by this wave alone
+#pragma unroll
+                for (int k = 0; k < KT; ++k) wu[first + k * S + mine][me] = s1[k], gate[first + k * S + mine][me] = s2[k];
+            };
+            if (here == 0) {
+                for (int e = lane; e < Q * 2 * NP; e += 64) red[wave * Q * 2 * NP + e] = 0.0f;
+            } else {
+#pragma unroll 1
+                for (int first = Q - HQ; first >= 0; first -= HQ) {
+                    if (marks == 0) sweep(std::false_type{}, first);
+                    else sweep(std::true_type{}, first);
                 }
             }
             __syncthreads();
+            if (t0 > t_begin) fetch(t0 - Q);
+            const ScanArgs r = scan_args();
+            if (quad_n > 0 && row0 + quad_unit < r.B) {
+                const int64_t quad_len = len[quad_unit], quad_0 = t0 + wave_t;
+                float dD[4], dbias[4];
+                load<float, 4>(sums[threadIdx.x], dD);
+                load<float, 4>(sums[TH + threadIdx.x], dbias);
+#pragma unroll
+                for (int k = 0; k < IT; ++k) {
+                    const int i = quad_t + k * STEP;
+                    const int64_t t = t0 + i;
+                    if (t < t_end) {
+                        const bool in = t < quad_len;
+                        float w[4], s1[4], s2[4], sy[4], ou[4], od[4], oz[4];
+                        load<float, 4>(&width[i][slot], w);
+                        load<float, 4>(&wu[i][slot], s1);
+                        load<float, 4>(&gate[i][slot], s2);
+                        load<float, 4>(&sum_y[i][slot], sy);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float skip = param[1][slot + j], uu = gu[k].at(j), out = gy[k].at(j), zz = gz[k].at(j);
+                            const float sg = sigmoid_f(zz), gg = gated ? out * (zz * sg) : out;
+                            ou[j] = in ? fmaf(s1[j], w[j], gg * skip) : 0.0f;
+                            // sum of through A = sum of through A2, times ln 2
+                            od[j] = in ? fmaf(s1[j], uu, s2[j] * kLn2) * step_slope(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
+                            oz[j] = in ? out * fmaf(skip, uu, sy[j]) * (sg * fmaf(zz, 1.0f - sg, 1.0f)) : 0.0f;
+                            dbias[j] += od[j];
+                            if (in) dD[j] = fmaf(gg, uu, dD[j]);
+                        }
+                        auto to = [&](void* base, int64_t row, int64_t token, const float(&v)[4]) {
+                            store4((T*)base + row0 * row + (quad_0 + k * STEP) * token + (int64_t)g * Dg + away(row, token), quad_n, whole, v);
+                        };
+                        to(r.du, r.du_row, r.du_token, ou);
+                        to(r.ddelta, r.ddelta_row, r.ddelta_token, od);
+                        if (gated) to(r.dz, r.dz_row, r.dz_token, oz);
+                    }
+                }
+                store<float, 4>(sums[threadIdx.x], dD);
+                store<float, 4>(sums[TH + threadIdx.x], dbias);
+            }
+            for (int e = thread_anew(); e < units * Q * 2 * NP; e += TH) {
+                const int un = e / (Q * 2 * NP), i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
+                const int64_t br = row0 + un, t = t0 + i;
+                if (br < r.B && t < t_end && s < N) {
+                    float sum = 0.0f;
+                    for (int w = 0; w < per; ++w) sum += red[((un * per + w) * Q + i) * 2 * NP + which * NP + s];
+                    if (r.bc_partial)
+                        r.bc_partial[((((int64_t)tb * r.B + br) * r.L + t) * r.G + g) * 2 * NP + which * NP + s] = sum;
+                    else if (which == 0)
+                        ((T*)r.dB + br * r.dB_row + t * r.dB_token + g * r.dB_group)[s] = (T)sum;
+                    else
+                        ((T*)r.dC + br * r.dC_row + t * r.dC_token + g * r.dC_group)[s] = (T)sum;
+                }
+            }
         }
+        const ScanArgs r = scan_args();
         if (MODE == 1) {
             if (live && on) {
-                const int64_t o = ((chunk * a.B + b) * a.D + d) * NP + q * 4;
+                const int64_t o = ((chunk * r.B + b) * r.D + d) * NP + q * 4;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    a.chunk_state[o + j] = carry[j];
-                    a.chunk_decay[o + j] = cut ? 0.0f : exp2_hw(sum_dt * A2[j]);
+                    r.chunk_state[o + j] = carry[j];
+                    r.chunk_decay[o + j] = cut ? 0.0f : exp2_hw(sum_dt * A2[j]);
                 }
             }
-        } else if (a.dstate && a.chunks == 1 && live && on) {
+        } else if (r.dstate && r.chunks == 1 && live && on) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (q * 4 + j < a.N) a.dstate[(b * a.D + d) * a.N + q * 4 + j] = carry[j];
+                if (q * 4 + j < N) r.dstate[(b * r.D + d) * N + q * 4 + j] = carry[j];
         }
     }
     if (MODE == 1) return;
-    if (working) {
-        const int64_t K = a.N + 2;
-        // the lanes of a channel finished different tokens: their dD and dbias add up
-        dD = lane_sum<0, SB>(dD);
-        dbias = lane_sum<0, SB>(dbias);
-        float* const rec = a.partial + (((int64_t)blockIdx.x * units + unit) * a.D + d) * K;
-        if (live) {
+    // this workgroup's record: dA from the sweeps' lanes; dD and ddelta_bias of the threads that share channels, in order
+    const int K = N + 2;
+    float* const rec = a.partial + (int64_t)blockIdx.x * units * a.D * K;
+    if (live) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (q * 4 + j < a.N) rec[q * 4 + j] = dA[j];
-            if (q == 0) {
-                rec[a.N] = dD;
-                rec[a.N + 1] = dbias;
-            }
+        for (int j = 0; j < 4; ++j)
+            if (q * 4 + j < N) rec[((int64_t)unit * a.D + d) * K + q * 4 + j] = dA[j];
+    }
+    __syncthreads();
+    if (quad_t == 0 && quad_n > 0) {
+        for (int j = 0; j < quad_n; ++j) {
+            float x = 0.0f, y = 0.0f;
+            for (int i = 0; i < STEP; ++i) x += sums[i * QUADS + threadIdx.x][j], y += sums[TH + i * QUADS + threadIdx.x][j];
+            rec[((int64_t)quad_unit * a.D + quad_d + j) * K + N] = x;
+            rec[((int64_t)quad_unit * a.D + quad_d + j) * K + N + 1] = y;
         }
     }
 }
@@ -524,7 +755,7 @@ __global__ __launch_bounds__(256) void k_scan_sum_bc(ScanArgs a, int NP, int blo
 // ----------------------------------------------------------------------------------------------------------------
 template <class T, int S, bool WHOLE>   // WHOLE: N = 4 S and everything a lane loads in fours is aligned for it
 __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
-    constexpr int SB = S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0;
+    constexpr int SB = lane_bits<S>();
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S;   // (row, channel)
     const int q = threadIdx.x % S;
     const bool live = i < a.B * a.D;
@@ -561,7 +792,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
         h[j] = fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[j], dt * u * Bv[j]);
         acc = fmaf(h[j], Cv[j], acc);
     }
-    acc = lane_sum<0, SB>(acc);
+    acc = lane_sum<SB>(acc);
     if (!live) return;
     if (WHOLE) store<float, 4>(a.new_state + o, h);
     else

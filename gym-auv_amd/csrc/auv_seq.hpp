@@ -45,10 +45,9 @@ __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(
 // part the rounding of the product alone costs |x| 2^-24 of relative error.
 __device__ __forceinline__ float exp_f(float x) {
     const float hi = x * kLog2e;
-    const float lo = fmaf(x, kLog2e, -hi) + x * kLog2eLow;
-    const float e = exp2_hw(hi);
-    // e = 0 and e = inf stand as they are (lo is NaN where hi is infinite)
-    return (e > 0.0f && e < __builtin_inff()) ? fmaf(e, lo * kLn2, e) : e;
+    // (infinite x: the low part is NaN, which the median of three turns into a finite number; e is then 0, infinite or NaN)
+    const float lo = __builtin_amdgcn_fmed3f(fmaf(x, kLog2eLow, fmaf(x, kLog2e, -hi)), -1.0f, 1.0f);
+    return exp2_hw(hi) * fmaf(lo, kLn2, 1.0f);
 }
 
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f(-x)); }
@@ -74,19 +73,148 @@ __device__ __forceinline__ float softplus_f(float x) {
     return (x < 0.0f ? 0.0f : x) + log1p_unit(e);
 }
 
-// One value passed within the wave to the lane whose number differs in bit `BIT`.
-template <int BIT>
-__device__ __forceinline__ float lane_xor(float x) {
-    return __shfl_xor(x, 1 << BIT, 64);
+// A value that is the same in every lane, as a scalar: what is computed from it needs no vector instructions.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Lane exchanges.  Within 16 lanes by data-parallel operands, which cost the instruction that uses them nothing; across
+// by the two instructions that swap halves of two registers.  No LDS traffic, unlike a general permutation.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-// Sum over the lanes that differ in bits LO .. HI-1, left in all of them.
-template <int LO, int HI>
+constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kQuadXor3 = 0x1b, kHalfMirror = 0x141, kMirror = 0x140, kRotate8 = 0x128;
+
+// After this, a holds both registers' low (BIT clear) parts side by side and b both high parts.
+template <int BIT>
+__device__ __forceinline__ void swap_halves(float& a, float& b) {
+    static_assert(BIT == 4 || BIT == 5, "rows of 16 or halves of 32 lanes");
+    const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+    if constexpr (BIT == 5) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        a = __builtin_bit_cast(float, (unsigned)r[0]), b = __builtin_bit_cast(float, (unsigned)r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        a = __builtin_bit_cast(float, (unsigned)r[0]), b = __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+}
+
+// Sum over the lanes that differ in bits 0 .. HI-1, left in all of them.  (Mirrors do for single bits: the lanes of the
+// lower bits already agree.)
+template <int HI>
 __device__ __forceinline__ float lane_sum(float x) {
-    if constexpr (LO < HI) {
-        x += lane_xor<LO>(x);
-        x = lane_sum<LO + 1, HI>(x);
+    if constexpr (HI > 0) x += dpp<kQuadXor1>(x);
+    if constexpr (HI > 1) x += dpp<kQuadXor2>(x);
+    if constexpr (HI > 2) x += dpp<kHalfMirror>(x);
+    if constexpr (HI > 3) x += dpp<kMirror>(x);
+    if constexpr (HI > 4) {
+        float y = x;
+        swap_halves<4>(x, y);
+        x += y;
+    }
+    if constexpr (HI > 5) {
+        float y = x;
+        swap_halves<5>(x, y);
+        x += y;
     }
     return x;
+}
+
+// r = a + a of the lane 8 (4) away in lanes 0-7 (0-3, 8-11) of each 16, and b + b of that lane in the others: an add that
+// writes only some banks of four lanes, so that a pair takes two instructions and no selects.  Four pairs at a time, which
+// keeps the two wait states between a register's write and its use as a shifted operand to one s_nop on either side.
+__device__ __forceinline__ void pair_sum8(float* v, int h) {
+    float r0, r1, r2, r3;
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %0, %8, %8 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %1, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %2, %10, %10 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %3, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "s_nop 1"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[h]), "v"(v[h + 1]), "v"(v[h + 2]), "v"(v[h + 3]));
+    v[0] = r0, v[1] = r1, v[2] = r2, v[3] = r3;
+}
+__device__ __forceinline__ void pair_sum4(float* v, int h) {
+    float r0, r1, r2, r3;
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %4, %4 row_shl:4 row_mask:0xf bank_mask:0x5\n\t"
+        "v_add_f32_dpp %1, %5, %5 row_shl:4 row_mask:0xf bank_mask:0x5\n\t"
+        "v_add_f32_dpp %2, %6, %6 row_shl:4 row_mask:0xf bank_mask:0x5\n\t"
+        "v_add_f32_dpp %3, %7, %7 row_shl:4 row_mask:0xf bank_mask:0x5\n\t"
+        "v_add_f32_dpp %0, %8, %8 row_shr:4 row_mask:0xf bank_mask:0xa\n\t"
+        "v_add_f32_dpp %1, %9, %9 row_shr:4 row_mask:0xf bank_mask:0xa\n\t"
+        "v_add_f32_dpp %2, %10, %10 row_shr:4 row_mask:0xf bank_mask:0xa\n\t"
+        "v_add_f32_dpp %3, %11, %11 row_shr:4 row_mask:0xf bank_mask:0xa\n\t"
+        "s_nop 1"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[h]), "v"(v[h + 1]), "v"(v[h + 2]), "v"(v[h + 3]));
+    v[0] = r0, v[1] = r1, v[2] = r2, v[3] = r3;
+}
+
+// One halving step of the sums below: v[0 .. H) become the sums over the lanes that differ in bit BIT, of v[0 .. H) where
+// that bit is clear and of v[H .. 2H) where it is set.
+template <int BIT, int H>
+__device__ __forceinline__ void halve(float* v) {
+    if constexpr ((BIT == 3 || BIT == 2) && H % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < H; i += 4) {
+            if constexpr (BIT == 3) pair_sum8(v + i, H);
+            else pair_sum4(v + i, H);
+        }
+    } else if constexpr (BIT >= 4) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            swap_halves<BIT>(v[i], v[i + H]);
+            v[i] += v[i + H];
+        }
+    } else {
+        const bool high = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) >> BIT & 1;
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float keep = high ? v[i + H] : v[i], give = high ? v[i] : v[i + H];
+            if constexpr (BIT == 3) v[i] = keep + dpp<kRotate8>(give);
+            else if constexpr (BIT == 2) v[i] = keep + dpp<kQuadXor3>(dpp<kHalfMirror>(give));   // 7-i, then 3-i: i xor 4
+            else if constexpr (BIT == 1) v[i] = keep + dpp<kQuadXor2>(give);
+            else v[i] = keep + dpp<kQuadXor1>(give);
+        }
+    }
+}
+
+// Sums of N values at once over the lanes that differ in some bits, each left in one lane only: with every bit the number
+// of values halves, so that they cost some 2 N instructions in place of N times the bits.  v[0 .. R) hold the sums, R = N
+// over the number of lanes (at least 1), and lane_place says which values' they are.  The bits whose steps are cheapest, 3
+// and 2, go first, while the values are many.
+template <int HI, int LO, int N>
+__device__ __forceinline__ void lane_scatter_sum(float* v) {
+    constexpr int order[6] = {3, 2, 5, 4, 1, 0};
+    constexpr auto count = [](int upto) {   // values left before step `upto`
+        int n = N;
+        for (int k = 0; k < upto; ++k)
+            if (order[k] < HI && order[k] >= LO && n > 1) n /= 2;
+        return n;
+    };
+    if constexpr (3 < HI && 3 >= LO && count(0) > 1) halve<3, count(0) / 2>(v);
+    if constexpr (2 < HI && 2 >= LO && count(1) > 1) halve<2, count(1) / 2>(v);
+    if constexpr (5 < HI && 5 >= LO && count(2) > 1) halve<5, count(2) / 2>(v);
+    if constexpr (4 < HI && 4 >= LO && count(3) > 1) halve<4, count(3) / 2>(v);
+    if constexpr (1 < HI && 1 >= LO && count(4) > 1) halve<1, count(4) / 2>(v);
+    if constexpr (0 < HI && 0 >= LO && count(5) > 1) halve<0, count(5) / 2>(v);
+}
+// The number of the first of the values whose sums lane_scatter_sum leaves in this lane.
+template <int HI, int LO, int N>
+__device__ __forceinline__ int lane_place(int lane) {
+    constexpr int order[6] = {3, 2, 5, 4, 1, 0};
+    int n = N, at = 0;
+    for (int k = 0; k < 6; ++k)
+        if (order[k] < HI && order[k] >= LO && n > 1) {
+            n /= 2;
+            if (lane >> order[k] & 1) at += n;
+        }
+    return at;
 }
 
 // dst[m] = sum over s of src[s * stride + m], in a fixed order: 32 partial sums of every 32nd slice, then those in
