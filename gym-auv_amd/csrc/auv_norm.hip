@@ -7,7 +7,11 @@ namespace auv {
 namespace seq {
 namespace {
 
-int64_t lanes_of(int64_t channels) { return channels <= 128 ? 16 : channels <= 512 ? 64 : channels <= 2048 ? 256 : 1024; }
+int64_t lanes_of(int64_t channels) {
+    for (int64_t lanes : {4, 8, 16, 32, 64, 256})
+        if (channels <= lanes * kNormLane) return lanes;
+    return 1024;
+}
 int64_t rows_of(int64_t lanes) { return lanes < 256 ? 256 / lanes : 1; }
 
 // Workgroups of a backward pass: each leaves one record of column sums, so a workgroup takes many rows.  2,048 of 256
@@ -30,14 +34,14 @@ int check(const auv_norm_args& p, int32_t pass) {
     return AUV_OK;
 }
 
-template <class TR, class T, int V, int TPR>
+template <class TR, class T, int TPR>
 int launch(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t blocks, hipStream_t stream) {
     constexpr int TH = norm_threads<TPR>();
     if (pass == AUV_SEQ_FORWARD) {
-        hipLaunchKernelGGL((k_norm_forward<TR, T, V, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
+        hipLaunchKernelGGL((k_norm_forward<TR, T, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
         return launched("k_norm_forward");
     }
-    hipLaunchKernelGGL((k_norm_backward<TR, T, V, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
+    hipLaunchKernelGGL((k_norm_backward<TR, T, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
     if (const int rc = launched("k_norm_backward")) return rc;
     if (!a.partial) return AUV_OK;
     SumArgs s{};
@@ -52,18 +56,16 @@ int launch(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t bloc
 }
 
 template <class TR, class T>
-int by_shape(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t blocks, int64_t V, hipStream_t stream) {
-    auto with = [&](auto width) {
-        constexpr int W = decltype(width)::value;
-        switch (lanes_of(p.channels)) {
-            case 16: return launch<TR, T, W, 16>(p, pass, a, blocks, stream);
-            case 64: return launch<TR, T, W, 64>(p, pass, a, blocks, stream);
-            case 256: return launch<TR, T, W, 256>(p, pass, a, blocks, stream);
-            default: return launch<TR, T, W, 1024>(p, pass, a, blocks, stream);
-        }
-    };
-    if (V >= 4) return with(std::integral_constant<int, 4>{});
-    return V == 2 ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 1>{});
+int by_shape(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t blocks, hipStream_t stream) {
+    switch (lanes_of(p.channels)) {
+        case 4: return launch<TR, T, 4>(p, pass, a, blocks, stream);
+        case 8: return launch<TR, T, 8>(p, pass, a, blocks, stream);
+        case 16: return launch<TR, T, 16>(p, pass, a, blocks, stream);
+        case 32: return launch<TR, T, 32>(p, pass, a, blocks, stream);
+        case 64: return launch<TR, T, 64>(p, pass, a, blocks, stream);
+        case 256: return launch<TR, T, 256>(p, pass, a, blocks, stream);
+        default: return launch<TR, T, 1024>(p, pass, a, blocks, stream);
+    }
 }
 }  // namespace
 }  // namespace seq
@@ -105,15 +107,6 @@ int auv_residual_norm(const auv_norm_args* p, int32_t pass, void* stream) {
     if (blocks > 0x7fffffff) return seq_fail(AUV_ERR_ARG, "auv_residual_norm: too many rows for one launch");
     if (sums && (!p->workspace || p->workspace_bytes < blocks * p->channels * 3 * (int64_t)sizeof(float)))
         return seq_fail(AUV_ERR_MEMORY, "auv_residual_norm: the workspace holds %lld bytes, too few", (long long)p->workspace_bytes);
-    const int64_t size = type_size(p->dtype), rsize = type_size(p->residual_dtype);
-    Width w(4);
-    w.stride(p->channels);
-    for (const void* q : {p->x, (const void*)p->x_out, p->d_x_out, (const void*)p->d_x}) w.pointer(q, rsize);
-    for (const void* q : {p->y, p->gate, (const void*)p->h, p->d_h, (const void*)p->d_y, (const void*)p->d_gate}) w.pointer(q, size);
-    for (int64_t s : {p->x_row, p->x_token, p->y_row, p->y_token, p->gate_row, p->gate_token, p->x_out_row, p->x_out_token, p->h_row,
-                      p->h_token, p->d_x_out_row, p->d_x_out_token, p->d_h_row, p->d_h_token, p->d_x_row, p->d_x_token, p->d_y_row,
-                      p->d_y_token, p->d_gate_row, p->d_gate_token})
-        w.stride(s);
     DeviceScope scope(p->device);
     if (!scope.ok()) return seq_fail(AUV_ERR_DEVICE, "auv_residual_norm: no HIP device %lld", (long long)p->device);
     NormArgs a{};
@@ -133,11 +126,10 @@ int auv_residual_norm(const auv_norm_args* p, int32_t pass, void* stream) {
     a.dgate = p->d_gate, a.dgate_row = p->d_gate_row, a.dgate_token = p->d_gate_token;
     a.partial = sums ? (float*)p->workspace : nullptr;
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t V = w.elements();
-    if (p->dtype == AUV_F32) return by_shape<float, float>(*p, pass, a, blocks, V, st);
+    if (p->dtype == AUV_F32) return by_shape<float, float>(*p, pass, a, blocks, st);
     if (p->dtype == AUV_BF16)
-        return p->residual_dtype == AUV_F32 ? by_shape<float, bf16>(*p, pass, a, blocks, V, st) : by_shape<bf16, bf16>(*p, pass, a, blocks, V, st);
-    return p->residual_dtype == AUV_F32 ? by_shape<float, f16>(*p, pass, a, blocks, V, st) : by_shape<f16, f16>(*p, pass, a, blocks, V, st);
+        return p->residual_dtype == AUV_F32 ? by_shape<float, bf16>(*p, pass, a, blocks, st) : by_shape<bf16, bf16>(*p, pass, a, blocks, st);
+    return p->residual_dtype == AUV_F32 ? by_shape<float, f16>(*p, pass, a, blocks, st) : by_shape<f16, f16>(*p, pass, a, blocks, st);
 }
 
 }  // extern "C"

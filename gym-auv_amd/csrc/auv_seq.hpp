@@ -12,12 +12,14 @@ namespace seq {
 using bf16 = __bf16;
 using f16 = _Float16;
 
+// V adjacent elements.  The hardware takes wide accesses at any address, so the type asks for no more alignment than an
+// element's: rows of an odd number of channels are read as wide as others.
 template <class T, int V>
-struct __attribute__((aligned(sizeof(T) * V))) Vec {
+struct __attribute__((packed, aligned(sizeof(T)))) Vec {
     T v[V];
 };
 
-// V elements of T as floats; the address must be a multiple of V * sizeof(T).
+// V elements of T as floats.
 template <class T, int V>
 __device__ __forceinline__ void load(const T* p, float (&out)[V]) {
     const Vec<T, V> t = *reinterpret_cast<const Vec<T, V>*>(p);
@@ -32,6 +34,52 @@ __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
     for (int i = 0; i < V; ++i) t.v[i] = (T)in[i];
     *reinterpret_cast<Vec<T, V>*>(p) = t;
 }
+
+// V adjacent elements as they lie in memory, in 32-bit words.  Taking the elements out, or merging them with the zeros of
+// a load left out, would wait for the load there and then; words wait until they are used.
+template <class T, int V>
+struct Raw {
+    static constexpr int kWords = (int)sizeof(T) * V / 4;
+    unsigned w[kWords];
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
+        else return (float)__builtin_bit_cast(T, (unsigned short)(w[i / 2] >> (16 * (i % 2))));
+    }
+};
+// The first `count` (0 to V) of V elements at p; the others come out as 0.
+template <class T, int V>
+__device__ __forceinline__ void fetch(Raw<T, V>& out, const T* p, int count) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        unsigned w[Raw<T, V>::kWords];
+    };
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::kWords; ++i) out.w[i] = 0;
+    if (count == V) {
+        const Words t = *reinterpret_cast<const Words*>(p);
+#pragma unroll
+        for (int i = 0; i < Raw<T, V>::kWords; ++i) out.w[i] = t.w[i];
+    } else if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i)
+            if (i < count) {
+                if constexpr (sizeof(T) == 4) out.w[i] = reinterpret_cast<const unsigned*>(p)[i];
+                else out.w[i / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i % 2));
+            }
+    }
+}
+// The first `count` of V elements to p.
+template <class T, int V>
+__device__ __forceinline__ void put(T* p, int count, const float (&in)[V]) {
+    if (count == V) {
+        store<T, V>(p, in);
+        asm volatile("");   // else the compiler shares this store's last element with the other branch, and splits it
+    } else {
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i)
+            if (i < count) p[i] = (T)in[i];
+    }
+}
+__device__ __forceinline__ int clamp_count(int64_t left, int most) { return left >= most ? most : left > 0 ? (int)left : 0; }
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eLow = (float)(1.44269504088896340736 - (double)kLog2e);
