@@ -24,38 +24,21 @@ int64_t conv_records(int64_t channels) {
 }
 
 struct Plan {
-    int64_t V, lanes, grid_x, grid_y;
+    int64_t lanes, grid_x, grid_y;
     int run;
 };
 
 Plan conv_plan(const auv_conv_args& p, int32_t pass) {
-    const int64_t size = type_size(p.dtype);
-    Width w(16 / size);
-    w.stride(p.channels);
-    w.pointer(p.x, size);
-    w.stride(p.x_row);
-    w.pointer(p.state, size);
-    w.pointer(p.new_state, size);
-    if (pass != AUV_SEQ_BACKWARD) {
-        w.pointer(p.y, size);
-        w.stride(p.y_row);
-    }
-    if (pass != AUV_SEQ_STEP) w.stride(p.x_token);
-    if (pass == AUV_SEQ_FORWARD) w.stride(p.y_token);
-    if (pass == AUV_SEQ_BACKWARD) {
-        for (const void* q : {p.d_y, p.d_new_state, (const void*)p.d_x, (const void*)p.d_state}) w.pointer(q, size);
-        for (int64_t s : {p.d_y_row, p.d_y_token, p.d_x_row, p.d_x_token}) w.stride(s);
-    }
+    const int64_t vectors = ceil_div(p.channels, 16 / type_size(p.dtype));
     Plan r;
-    r.V = w.elements();
-    const int64_t vectors = p.channels / r.V;
     r.run = conv_run(p.batch, p.length, vectors);
     r.lanes = vectors < kConvThreads ? vectors : kConvThreads;
     r.grid_y = ceil_div(vectors, r.lanes);
     const int64_t slots = kConvThreads / r.lanes;
     const int64_t want = ceil_div(p.batch * ceil_div(p.length, r.run), slots);
-    // forwards: a workgroup per set of runs; backwards a workgroup takes several, because each leaves a record of sums
-    const int64_t cap = pass == AUV_SEQ_BACKWARD ? conv_records(p.channels) : (int64_t)1 << 22;
+    // forwards: a workgroup per set of runs; backwards a workgroup takes several, because each leaves a record of sums;
+    // a step's takes several rows, because it loads its taps first
+    const int64_t cap = pass == AUV_SEQ_BACKWARD ? conv_records(p.channels) : pass == AUV_SEQ_STEP ? 1024 : (int64_t)1 << 22;
     r.grid_x = want < cap ? want : cap;
     return r;
 }
@@ -66,25 +49,24 @@ int check(const auv_conv_args& p, int32_t pass) {
     if (const int rc = check_rows(who, p.batch, p.length, p.channels, p.device, p.dtype)) return rc;
     if (p.width < 2 || p.width > 4) return seq_fail(AUV_ERR_ARG, "%s: width must be 2, 3 or 4, got %lld", who, (long long)p.width);
     if (pass == AUV_SEQ_STEP && p.length != 1) return seq_fail(AUV_ERR_ARG, "%s: a step takes one token per row", who);
-    if (p.channels > (int64_t)256 * 8 * 65535) return seq_fail(AUV_ERR_ARG, "%s: too many channels", who);
+    if (p.channels > (int64_t)256 * 4 * 65535) return seq_fail(AUV_ERR_ARG, "%s: too many channels", who);
     return AUV_OK;
 }
 
-template <class T, int W, int V>
+template <class T, int W>
 int launch(const auv_conv_args& p, int32_t pass, const Plan& r, ConvArgs a, hipStream_t stream) {
     const dim3 grid((unsigned)r.grid_x, (unsigned)r.grid_y), block(kConvThreads);
     if (pass == AUV_SEQ_FORWARD) {
-        hipLaunchKernelGGL((k_conv_forward<T, W, V>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_conv_forward<T, W>), grid, block, 0, stream, a);
         return launched("k_conv_forward");
     }
     if (pass == AUV_SEQ_STEP) {
-        const int64_t blocks = ceil_div(p.batch * (p.channels / V), kConvThreads);
-        if (blocks > 0x7fffffff) return seq_fail(AUV_ERR_ARG, "auv_causal_conv: batch too large for one launch");
-        hipLaunchKernelGGL((k_conv_step<T, W, V>), dim3((unsigned)blocks), block, 0, stream, a);
+        hipLaunchKernelGGL((k_conv_step<T, W>), grid, block, 0, stream, a);
         return launched("k_conv_step");
     }
+    constexpr int V = conv_vector<T>();
     const size_t lds = (size_t)(kConvThreads / r.lanes) * r.lanes * V * (W + 1) * sizeof(float);
-    hipLaunchKernelGGL((k_conv_backward<T, W, V>), grid, block, lds, stream, a);
+    hipLaunchKernelGGL((k_conv_backward<T, W>), grid, block, lds, stream, a);
     if (const int rc = launched("k_conv_backward")) return rc;
     if (!a.partial) return AUV_OK;
     SumArgs s{};
@@ -101,18 +83,9 @@ int launch(const auv_conv_args& p, int32_t pass, const Plan& r, ConvArgs a, hipS
 }
 
 template <class T>
-int by_shape(const auv_conv_args& p, int32_t pass, const Plan& r, const ConvArgs& a, hipStream_t stream) {
-    constexpr int kMost = 16 / (int)sizeof(T);
-    auto with_width = [&](auto width) {
-        constexpr int W = decltype(width)::value;
-        if constexpr (kMost >= 8)
-            if (r.V == 8) return launch<T, W, 8>(p, pass, r, a, stream);
-        if (r.V >= 4) return launch<T, W, 4>(p, pass, r, a, stream);
-        return r.V == 2 ? launch<T, W, 2>(p, pass, r, a, stream) : launch<T, W, 1>(p, pass, r, a, stream);
-    };
-    if (p.width == 2) return with_width(std::integral_constant<int, 2>{});
-    if (p.width == 3) return with_width(std::integral_constant<int, 3>{});
-    return with_width(std::integral_constant<int, 4>{});
+int by_width(const auv_conv_args& p, int32_t pass, const Plan& r, const ConvArgs& a, hipStream_t stream) {
+    if (p.width == 2) return launch<T, 2>(p, pass, r, a, stream);
+    return p.width == 3 ? launch<T, 3>(p, pass, r, a, stream) : launch<T, 4>(p, pass, r, a, stream);
 }
 }  // namespace
 
@@ -136,9 +109,7 @@ int64_t auv_causal_conv_workspace(const auv_conv_args* p, int32_t pass) {
     if (!p) return seq_fail(AUV_ERR_ARG, "auv_causal_conv_workspace: null argument");
     if (const int rc = check(*p, pass)) return rc;
     if (pass != AUV_SEQ_BACKWARD || p->batch == 0 || p->length == 0) return 0;
-    // the number of records follows from the access width, and that from the addresses: room for any
-    const int64_t runs = p->batch * ceil_div(p->length, 8), most = conv_records(p->channels);
-    return (runs < most ? runs : most) * p->channels * (p->width + 1) * (int64_t)sizeof(float);
+    return conv_plan(*p, pass).grid_x * p->channels * (p->width + 1) * (int64_t)sizeof(float);
 }
 
 int auv_causal_conv(const auv_conv_args* p, int32_t pass, void* stream) {
@@ -178,8 +149,8 @@ int auv_causal_conv(const auv_conv_args* p, int32_t pass, void* stream) {
     a.silu = p->silu != 0;
     a.run = r.run, a.lanes = (int32_t)r.lanes;
     const hipStream_t st = (hipStream_t)stream;
-    if (p->dtype == AUV_F32) return by_shape<float>(*p, pass, r, a, st);
-    return p->dtype == AUV_BF16 ? by_shape<bf16>(*p, pass, r, a, st) : by_shape<f16>(*p, pass, r, a, st);
+    if (p->dtype == AUV_F32) return by_width<float>(*p, pass, r, a, st);
+    return p->dtype == AUV_BF16 ? by_width<bf16>(*p, pass, r, a, st) : by_width<f16>(*p, pass, r, a, st);
 }
 
 }  // extern "C"
