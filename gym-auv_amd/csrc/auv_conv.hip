@@ -24,13 +24,15 @@ int64_t conv_records(int64_t channels) {
 }
 
 struct Plan {
-    int64_t lanes, grid_x, grid_y;
+    int64_t V, lanes, grid_x, grid_y;
     int run;
 };
 
 Plan conv_plan(const auv_conv_args& p, int32_t pass) {
-    const int64_t vectors = ceil_div(p.channels, 16 / type_size(p.dtype));
     Plan r;
+    r.V = 16 / type_size(p.dtype);
+    if (pass != AUV_SEQ_STEP && p.channels < r.V) r.V = 1;
+    const int64_t vectors = ceil_div(p.channels, r.V);
     r.run = conv_run(p.batch, p.length, vectors);
     r.lanes = vectors < kConvThreads ? vectors : kConvThreads;
     r.grid_y = ceil_div(vectors, r.lanes);
@@ -53,20 +55,19 @@ int check(const auv_conv_args& p, int32_t pass) {
     return AUV_OK;
 }
 
-template <class T, int W>
+template <class T, int W, int V>
 int launch(const auv_conv_args& p, int32_t pass, const Plan& r, ConvArgs a, hipStream_t stream) {
     const dim3 grid((unsigned)r.grid_x, (unsigned)r.grid_y), block(kConvThreads);
     if (pass == AUV_SEQ_FORWARD) {
-        hipLaunchKernelGGL((k_conv_forward<T, W>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_conv_forward<T, W, V>), grid, block, 0, stream, a);
         return launched("k_conv_forward");
     }
     if (pass == AUV_SEQ_STEP) {
         hipLaunchKernelGGL((k_conv_step<T, W>), grid, block, 0, stream, a);
         return launched("k_conv_step");
     }
-    constexpr int V = conv_vector<T>();
     const size_t lds = (size_t)(kConvThreads / r.lanes) * r.lanes * V * (W + 1) * sizeof(float);
-    hipLaunchKernelGGL((k_conv_backward<T, W>), grid, block, lds, stream, a);
+    hipLaunchKernelGGL((k_conv_backward<T, W, V>), grid, block, lds, stream, a);
     if (const int rc = launched("k_conv_backward")) return rc;
     if (!a.partial) return AUV_OK;
     SumArgs s{};
@@ -82,10 +83,14 @@ int launch(const auv_conv_args& p, int32_t pass, const Plan& r, ConvArgs a, hipS
     return launched("k_seq_sum");
 }
 
+template <class T, int W>
+int by_vector(const auv_conv_args& p, int32_t pass, const Plan& r, const ConvArgs& a, hipStream_t stream) {
+    return r.V == 1 ? launch<T, W, 1>(p, pass, r, a, stream) : launch<T, W, conv_vector<T>()>(p, pass, r, a, stream);
+}
 template <class T>
 int by_width(const auv_conv_args& p, int32_t pass, const Plan& r, const ConvArgs& a, hipStream_t stream) {
-    if (p.width == 2) return launch<T, 2>(p, pass, r, a, stream);
-    return p.width == 3 ? launch<T, 3>(p, pass, r, a, stream) : launch<T, 4>(p, pass, r, a, stream);
+    if (p.width == 2) return by_vector<T, 2>(p, pass, r, a, stream);
+    return p.width == 3 ? by_vector<T, 3>(p, pass, r, a, stream) : by_vector<T, 4>(p, pass, r, a, stream);
 }
 }  // namespace
 

@@ -39,7 +39,8 @@ __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
 // a load left out, would wait for the load there and then; words wait until they are used.
 template <class T, int V>
 struct Raw {
-    static constexpr int kWords = (int)sizeof(T) * V / 4;
+    static_assert(V == 1 || sizeof(T) * V % 4 == 0, "whole words, or one element");
+    static constexpr int kWords = ((int)sizeof(T) * V + 3) / 4;
     unsigned w[kWords];
     __device__ __forceinline__ float at(int i) const {
         if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
@@ -54,7 +55,9 @@ __device__ __forceinline__ void fetch(Raw<T, V>& out, const T* p, int count) {
     };
 #pragma unroll
     for (int i = 0; i < Raw<T, V>::kWords; ++i) out.w[i] = 0;
-    if (count == V) {
+    if constexpr (sizeof(T) * V == 2) {
+        if (count) out.w[0] = *reinterpret_cast<const unsigned short*>(p);
+    } else if (count == V) {
         const Words t = *reinterpret_cast<const Words*>(p);
 #pragma unroll
         for (int i = 0; i < Raw<T, V>::kWords; ++i) out.w[i] = t.w[i];
