@@ -227,12 +227,12 @@ def load():
     lib.auv_seq_last_error.restype = C.c_char_p
     lib.auv_seq_last_error.argtypes = []
     lib.auv_selective_scan_segments.restype = i64
-    lib.auv_selective_scan_segments.argtypes = [C.POINTER(AuvScanArgs)]
-    for name, args in (("auv_causal_conv", AuvConvArgs), ("auv_selective_scan", AuvScanArgs), ("auv_residual_norm", AuvNormArgs)):
+    lib.auv_selective_scan_segments.argtypes = [vp]
+    for name in ("auv_causal_conv", "auv_selective_scan", "auv_residual_norm"):   # blocks: Auv*Args, or their packed bytes
         call, room = getattr(lib, name), getattr(lib, name + "_workspace")
         call.restype = C.c_int
-        call.argtypes = [C.POINTER(args), i32, vp]
+        call.argtypes = [vp, i32, vp]
         room.restype = i64
-        room.argtypes = [C.POINTER(args), i32]
+        room.argtypes = [vp, i32]
     _lib = lib
     return lib

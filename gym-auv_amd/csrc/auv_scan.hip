@@ -171,7 +171,8 @@ int run_step(const ScanArgs& a, hipStream_t stream) {
     Width whole(4);
     whole.pointer(a.Bm, sizeof(T));
     whole.pointer(a.Cm, sizeof(T));
-    for (int64_t s : {a.B_row, a.B_group, a.C_row, a.C_group}) whole.stride(s);
+    if (a.B > 1) whole.stride(a.B_row), whole.stride(a.C_row);
+    if (a.G > 1) whole.stride(a.B_group), whole.stride(a.C_group);
     for (const float* q : {a.A, a.state, (const float*)a.new_state}) whole.pointer(q, 4);
     const dim3 grid((unsigned)ceil_div(a.B * a.D * S, 256)), block(256);
     if (a.N == 4 * S && whole.elements() == 4)
@@ -210,9 +211,10 @@ int by_states(const auv_scan_args& p, int32_t pass, ScanArgs a, hipStream_t stre
     Width fours(4);
     fours.stride(a.D / a.G);
     for (const void* q : {a.u, a.delta, a.z, a.dy, (const void*)a.du, (const void*)a.ddelta, (const void*)a.dz}) fours.pointer(q, sizeof(T));
-    for (int64_t s : {a.u_row, a.u_token, a.delta_row, a.delta_token, a.z_row, a.z_token, a.dy_row, a.dy_token, a.du_row, a.du_token,
-                      a.ddelta_row, a.ddelta_token, a.dz_row, a.dz_token})
-        fours.stride(s);
+    if (a.B > 1)
+        for (int64_t s : {a.u_row, a.delta_row, a.z_row, a.dy_row, a.du_row, a.ddelta_row, a.dz_row}) fours.stride(s);
+    if (a.L > 1)
+        for (int64_t s : {a.u_token, a.delta_token, a.z_token, a.dy_token, a.du_token, a.ddelta_token, a.dz_token}) fours.stride(s);
     a.whole = fours.elements() == 4;
     a.chunk = r.chunks.length, a.chunks = r.chunks.count;
     char* w = (char*)p.workspace;

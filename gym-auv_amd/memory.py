@@ -32,6 +32,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
+import weakref
 
 import torch
 import torch.nn as nn
@@ -49,161 +51,198 @@ WIDTHS = (2, 3, 4)
 # ----------------------------------------------------------------------------
 # checks
 # ----------------------------------------------------------------------------
-def _activation(name, t, shape=None, like=None):
-    """`t` is a float CUDA tensor with adjacent channels, of `shape`, and of `like`'s type and device."""
+# A call on a single vessel takes the GPU some 3 us, so the host's part counts: each check returns what the call goes on
+# to use, and the argument blocks (include/auvsim.h: 64-bit fields only) are packed in one go.
+
+def _first(name, t, dims, what):
+    """The tensor that fixes a call's type and device: (shape, strides, device number)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in TYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
-        if t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {like.device}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, strides = tuple(t.shape), t.stride()
+    if dims is not None and len(shape) != dims:
+        raise ValueError(f"{name} must be {what}, got {shape}")
+    if not shape:
+        raise ValueError(f"{name} must have a channel dimension")
+    if shape[-1] > 1 and strides[-1] != 1:
         raise ValueError(f"{name}: the last dimension must be adjacent in memory (call .contiguous())")
+    return shape, strides, t.get_device()
 
 
-def _dense(name, t, shape, like, dtype=torch.float32):
-    """An optional contiguous tensor of `dtype` (parameters, states, lengths)."""
-    if t is None:
-        return
+def _like(name, t, shape, dtype, dev):
+    """Strides of another activation of the call."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {like.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: the last dimension must be adjacent in memory (call .contiguous())")
+    return strides
+
+
+def _dense(name, t, shape, dev, dtype=torch.float32):
+    """Address of an optional contiguous tensor (parameters, states, lengths); 0 for None."""
+    if t is None:
+        return 0
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{dev}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
-def _marks(name, t, shape, like):
+def _marks(t, shape, dev):
+    """(address, row stride, token stride) of the optional start marks."""
     if t is None:
-        return
+        return 0, 0, 0
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bool, torch.uint8):
-        raise TypeError(f"{name} must be a bool or uint8 tensor")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {like.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        raise TypeError("start must be a bool or uint8 tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"start is on {t.device}, the call's other tensors on cuda:{dev}")
+    if t.shape != shape:
+        raise ValueError(f"start must be {tuple(shape)}, got {tuple(t.shape)}")
+    strides = t.stride()
+    return t.data_ptr(), strides[0], strides[1] if len(strides) > 1 else 0
 
 
-def _written(name, t, *others):
-    """`t` is written element by element: no two of its elements may share memory, and none may lie in `others`."""
-    if t.numel() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-        raise ValueError(f"{name} is written and must not be an expanded tensor")
-    lo, hi = _span(t)
-    for other_name, o in others:
-        if o is not None and o.numel() and t.numel():
-            a, b = _span(o)
-            if lo < b and a < hi:
-                raise ValueError(f"{name} overlaps {other_name}")
+def _apart(name, t, other_name, o):
+    """`t`, contiguous and about to be written, shares no memory with `o`."""
+    lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+    first = o.data_ptr()
+    last = first + (sum((n - 1) * s for n, s in zip(o.shape, o.stride())) + 1) * o.element_size() if o.numel() else first
+    if lo < last and first < hi:
+        raise ValueError(f"{name} overlaps {other_name}")
 
 
-def _span(t):
-    """First byte and the byte behind the last of a tensor's elements."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _wants_grad(tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _no_grad_here(who, *tensors):
-    if _wants_grad(*tensors):
+def _no_grad_here(who, tensors):
+    if _wants_grad(tensors):
         raise RuntimeError(f"{who} keeps no gradients: call it under torch.no_grad(), or use the form for whole rollouts")
 
 
-def _guard_capture(*leaves):
+class _EagerGraph:
+    """Lives as long as the graph node of an eager call; names the leaves it accumulates into (which the node keeps alive)."""
+    __slots__ = ("leaves", "__weakref__")
+
+    def __init__(self, leaves):
+        self.leaves = leaves
+
+
+_eager_graphs = weakref.WeakSet()
+
+
+def _mark_graph(tensors):
     """Refuse to record a graph whose backward pass would end in gradient accumulators that an eager graph made: torch
-    runs those on the eager graph's stream, and joining that stream to a capture ends the process.  An accumulator lives
-    as long as some graph uses it and carries a note of ours when that graph was made eagerly.  The caller holds what
-    this returns until its own graph does."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t is not None and t.requires_grad and t.is_leaf]
-    for node in nodes:
-        if not capturing:
-            node.metadata["auv_eager"] = True
-        elif "auv_eager" in node.metadata:
+    runs those on the eager graph's stream, and joining that stream to a capture ends the process.  Returns what the
+    call's own node is to keep."""
+    leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
+    if torch.cuda.is_current_stream_capturing():
+        if any(leaves & g.leaves for g in list(_eager_graphs)):
             raise RuntimeError("a graph that records gradients is being captured while the outputs of an earlier eager pass "
                                "over the same parameters are alive: drop those first")
-    return nodes
+        return None
+    mark = _EagerGraph(leaves)
+    _eager_graphs.add(mark)
+    return mark
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _strides(name, t, *dims):
-    """{name: pointer, name_row: stride, ...} of an activation; a dimension of one element has no stride to heed."""
+def _rows(t):
+    """(address, row stride, token stride) of an activation of our own making or known to be in order."""
     if t is None:
-        return {}
-    out = {name: t.data_ptr()}
-    for k, d in enumerate(dims):
-        out[f"{name}_{('row', 'token', 'group')[k]}"] = t.stride(d) if t.shape[d] > 1 else 0
-    return out
+        return 0, 0, 0
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1]
 
 
-def _call(name, args, what, device):
-    """Runs entry point `name` on the current stream with the scratch memory it asks for."""
-    lib = _lib.load()
-    ref = C.byref(args)
-    room = 0
-    if what == _lib.SEQ_BACKWARD or (what == _lib.SEQ_FORWARD and name == "auv_selective_scan"):
-        room = getattr(lib, name + "_workspace")(ref, what)
-        if room < 0:
-            raise _lib.AuvError(room, lib.auv_seq_last_error().decode())
-    scratch = None
-    if room:
-        scratch = torch.empty(room, dtype=torch.uint8, device=device)   # the stream's own: free for it again on return
-        args.workspace, args.workspace_bytes = scratch.data_ptr(), room
-    rc = getattr(lib, name)(ref, what, torch.cuda.current_stream(device).cuda_stream)
-    if rc != 0:
-        raise _lib.AuvError(rc, lib.auv_seq_last_error().decode())
+def _groups(t):
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1], s[2]
 
 
 def _adjacent(t):
     return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _packer(cls):
+    """Packs an argument block without its last two fields, the workspace's."""
+    kinds = {C.c_void_p: "q", C.c_int64: "q", C.c_double: "d"}
+    return struct.Struct("<" + "".join(kinds[k] for _, k in cls._fields_[:-2])).pack
+
+
+_pack_conv, _pack_scan, _pack_norm = _packer(_lib.AuvConvArgs), _packer(_lib.AuvScanArgs), _packer(_lib.AuvNormArgs)
+_pack_room = struct.Struct("<2q").pack
+_NO_ROOM = _pack_room(0, 0)
+
+
+def _call(name, block, what, dev, scratch=True):
+    """Runs entry point `name` on the current stream, with the scratch memory it asks for."""
+    lib = _lib.load()
+    tail = _NO_ROOM
+    if scratch:
+        room = getattr(lib, name + "_workspace")(block + _NO_ROOM, what)
+        if room < 0:
+            raise _lib.AuvError(room, lib.auv_seq_last_error().decode())
+        if room:
+            held = torch.empty(room, dtype=torch.uint8, device=dev)   # the stream's own: free for it again on return
+            tail = _pack_room(held.data_ptr(), room)
+    rc = getattr(lib, name)(block + tail, what, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != 0:
+        raise _lib.AuvError(rc, lib.auv_seq_last_error().decode())
+
+
 # ----------------------------------------------------------------------------
 # short causal convolution
 # ----------------------------------------------------------------------------
-def _conv_args(x, weight, bias, start, lengths, state, silu):
+def _conv_head(x, weight, bias, start, lengths, state, silu):
+    """The argument block up to state."""
     B, L, D = x.shape
-    return _lib.AuvConvArgs(device=x.device.index, dtype=TYPES[x.dtype], batch=B, length=L, channels=D, width=weight.shape[1],
-                            silu=bool(silu), weight=weight.data_ptr(), bias=_ptr(bias), lengths=_ptr(lengths), state=_ptr(state),
-                            **_strides("x", x, 0, 1), **_strides("start", start, 0, 1))
+    return (x.get_device(), TYPES[x.dtype], B, L, D, weight.shape[1], silu, *_rows(x), weight.data_ptr(), _ptr(bias), *_rows(start),
+            _ptr(lengths), _ptr(state))
 
 
 def _conv_forward(x, weight, bias, start, lengths, state, silu, return_state):
-    B, L, D = x.shape
     y = torch.empty_like(x)
-    new_state = torch.empty((B, weight.shape[1] - 1, D), dtype=x.dtype, device=x.device) if return_state else None
+    new = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if return_state else None
     if x.numel() == 0:
         if return_state:
-            new_state.copy_(state) if state is not None else new_state.zero_()
-        return y, new_state
-    a = _conv_args(x, weight, bias, start, lengths, state, silu)
-    a.y, a.y_row, a.y_token, a.new_state = y.data_ptr(), y.stride(0), y.stride(1), _ptr(new_state)
-    _call("auv_causal_conv", a, _lib.SEQ_FORWARD, x.device)
-    return y, new_state
+            new.copy_(state) if state is not None else new.zero_()
+        return y, new
+    head = _conv_head(x, weight, bias, start, lengths, state, silu)
+    _call("auv_causal_conv", _pack_conv(*head, _ptr(new), *_rows(y), *(0,) * 10), _lib.SEQ_FORWARD, head[0], scratch=False)
+    return y, new
 
 
 class _Conv(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, state, start, lengths, silu, return_state):
+    def forward(ctx, x, weight, bias, state, start, lengths, silu, return_state, mark):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, state, start, lengths)
-        ctx.silu = silu
+        ctx.silu, ctx.mark = silu, mark
         return _conv_forward(x, weight, bias, start, lengths, state, silu, return_state)
 
     @staticmethod
@@ -211,30 +250,31 @@ class _Conv(torch.autograd.Function):
     def backward(ctx, dy, dnew):
         x, weight, bias, state, start, lengths = ctx.saved_tensors
         want_x, want_w, want_b, want_s = ctx.needs_input_grad[:4]
+        rest = (None,) * 5
         if x.numel() == 0:
             zeros = lambda t, want: torch.zeros_like(t) if want else None   # noqa: E731
             ds = None if not want_s else torch.zeros_like(state) if dnew is None else dnew.clone()
-            return zeros(x, want_x), zeros(weight, want_w), zeros(bias, want_b), ds, None, None, None, None
+            return (zeros(x, want_x), zeros(weight, want_w), zeros(bias, want_b), ds) + rest
         dy = torch.zeros_like(x) if dy is None else _adjacent(dy)
         dnew = None if dnew is None else dnew.contiguous()
         dx = torch.empty_like(x)
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(bias) if want_b else None
         ds = torch.empty_like(state) if want_s else None
-        a = _conv_args(x, weight, bias, start, lengths, state, ctx.silu)
-        a.d_y, a.d_y_row, a.d_y_token = dy.data_ptr(), dy.stride(0), dy.stride(1)
-        a.d_x, a.d_x_row, a.d_x_token = dx.data_ptr(), dx.stride(0), dx.stride(1)
-        a.d_new_state, a.d_weight, a.d_bias, a.d_state = _ptr(dnew), _ptr(dw), _ptr(db), _ptr(ds)
-        _call("auv_causal_conv", a, _lib.SEQ_BACKWARD, x.device)
-        return dx if want_x else None, dw, db, ds, None, None, None, None
+        head = _conv_head(x, weight, bias, start, lengths, state, ctx.silu)
+        block = _pack_conv(*head, 0, 0, 0, 0, *_rows(dy), _ptr(dnew), *_rows(dx), _ptr(dw), _ptr(db), _ptr(ds))
+        _call("auv_causal_conv", block, _lib.SEQ_BACKWARD, head[0])
+        return (dx if want_x else None, dw, db, ds) + rest
 
 
-def _check_conv(x, weight, bias):
-    D = x.shape[-1]
+def _taps(weight, bias, D, dev):
+    """The width, of taps in order."""
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] not in WIDTHS:
         raise ValueError(f"weight must be [channels, width] with a width of {WIDTHS}")
-    _dense("weight", weight, (D, weight.shape[1]), x)
-    _dense("bias", bias, (D,), x)
+    W = weight.shape[1]
+    _dense("weight", weight, (D, W), dev)
+    _dense("bias", bias, (D,), dev)
+    return W
 
 
 def causal_conv(x, weight, bias=None, *, start=None, lengths=None, state=None, silu=True, return_state=False):
@@ -245,17 +285,14 @@ def causal_conv(x, weight, bias=None, *, start=None, lengths=None, state=None, s
     type holds the tokens before the row (None: zeros).  With return_state also the state
     behind each row's last token, which `causal_conv_step` goes on from.  Differentiable in
     x, weight, bias and state."""
-    _activation("x", x)
-    if x.dim() != 3:
-        raise ValueError(f"x must be [batch, length, channels], got {tuple(x.shape)}")
-    B, L, D = x.shape
-    _check_conv(x, weight, bias)
-    _marks("start", start, (B, L), x)
-    _dense("lengths", lengths, (B,), x, torch.int32)
-    _dense("state", state, (B, weight.shape[1] - 1, D), x, x.dtype)
-    if _wants_grad(x, weight, bias, state):
-        held = _guard_capture(x, weight, bias, state)   # noqa: F841
-        y, new = _Conv.apply(x, weight, bias, state, start, lengths, bool(silu), bool(return_state))
+    (B, L, D), _, dev = _first("x", x, 3, "[batch, length, channels]")
+    W = _taps(weight, bias, D, dev)
+    _marks(start, (B, L), dev)
+    _dense("lengths", lengths, (B,), dev, torch.int32)
+    _dense("state", state, (B, W - 1, D), dev, x.dtype)
+    silu, tensors = 1 if silu else 0, (x, weight, bias, state)
+    if _wants_grad(tensors):
+        y, new = _Conv.apply(*tensors, start, lengths, silu, bool(return_state), _mark_graph(tensors))
     else:
         y, new = _conv_forward(x, weight, bias, start, lengths, state, silu, return_state)
     return (y, new) if return_state else y
@@ -264,118 +301,116 @@ def causal_conv(x, weight, bias=None, *, start=None, lengths=None, state=None, s
 def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_state=None):
     """`causal_conv` of one token per row: x [batch, channels] -> y [batch, channels].  `state`
     [batch, width-1, channels] moves up by the token, in place or into `new_state`."""
-    _activation("x", x)
-    if x.dim() != 2:
-        raise ValueError(f"x must be [batch, channels], got {tuple(x.shape)}")
-    B, D = x.shape
-    _check_conv(x, weight, bias)
+    (B, D), strides, dev = _first("x", x, 2, "[batch, channels]")
+    W = _taps(weight, bias, D, dev)
     if state is None:
         raise TypeError("state must be a tensor, got None")
-    shape = (B, weight.shape[1] - 1, D)
-    _dense("state", state, shape, x, x.dtype)
-    _marks("start", start, (B,), x)
-    _no_grad_here("causal_conv_step", x, state, weight, bias)
-    if new_state is None:
-        new_state = state
-    elif new_state is not state:
-        _dense("new_state", new_state, shape, x, x.dtype)
-        _written("new_state", new_state, ("state", state), ("x", x))
+    s = _dense("state", state, (B, W - 1, D), dev, x.dtype)
+    marks = _marks(start, (B,), dev)
+    _no_grad_here("causal_conv_step", (x, state, weight, bias))
+    to = s
+    if new_state is not None and new_state is not state:
+        to = _dense("new_state", new_state, (B, W - 1, D), dev, x.dtype)
+        _apart("new_state", new_state, "state", state)
+        _apart("new_state", new_state, "x", x)
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    if x.numel() == 0:
-        return y
-    a = _lib.AuvConvArgs(device=x.device.index, dtype=TYPES[x.dtype], batch=B, length=1, channels=D, width=shape[1] + 1,
-                         silu=bool(silu), weight=weight.data_ptr(), bias=_ptr(bias), state=state.data_ptr(),
-                         new_state=new_state.data_ptr(), y=y.data_ptr(), y_row=D, **_strides("x", x, 0), **_strides("start", start, 0))
-    _call("auv_causal_conv", a, _lib.SEQ_STEP, x.device)
+    if B and D:
+        block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
+                           _ptr(bias), *marks, 0, s, to, y.data_ptr(), D, 0, *(0,) * 10)
+        _call("auv_causal_conv", block, _lib.SEQ_STEP, dev, scratch=False)
     return y
 
 
 # ----------------------------------------------------------------------------
 # selective state space scan
 # ----------------------------------------------------------------------------
-def _scan_args(u, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, softplus):
-    B, L, Dc = u.shape
-    return _lib.AuvScanArgs(device=u.device.index, dtype=TYPES[u.dtype], batch=B, length=L, channels=Dc, states=A.shape[1],
-                            groups=Bm.shape[2], softplus=bool(softplus), A=A.data_ptr(), D=_ptr(D), delta_bias=_ptr(delta_bias),
-                            lengths=_ptr(lengths), state=_ptr(state), **_strides("u", u, 0, 1), **_strides("delta", delta, 0, 1),
-                            **_strides("z", z, 0, 1), **_strides("B", Bm, 0, 1, 2), **_strides("C", Cm, 0, 1, 2),
-                            **_strides("start", start, 0, 1))
-
-
-def _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, softplus, return_state, keep):
+def _scan_forward(u, A, state, head, return_state, keep):
+    """`head`: the argument block up to state."""
     y = torch.empty_like(u)
-    new_state = torch.empty((u.shape[0],) + tuple(A.shape), dtype=torch.float32, device=u.device) if return_state else None
+    new = torch.empty((u.shape[0],) + tuple(A.shape), dtype=torch.float32, device=u.device) if return_state else None
     if u.numel() == 0:
         if return_state:
-            new_state.copy_(state) if state is not None else new_state.zero_()
-        return y, new_state, None
-    a = _scan_args(u, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, softplus)
-    a.y, a.y_row, a.y_token, a.new_state = y.data_ptr(), y.stride(0), y.stride(1), _ptr(new_state)
+            new.copy_(state) if state is not None else new.zero_()
+        return y, new, None
     segments = None
     if keep:
-        n = _lib.load().auv_selective_scan_segments(C.byref(a))
+        lib = _lib.load()
+        n = lib.auv_selective_scan_segments(_pack_scan(*head, *(0,) * 30) + _NO_ROOM)
         if n < 0:
-            raise _lib.AuvError(n, _lib.load().auv_seq_last_error().decode())
+            raise _lib.AuvError(n, lib.auv_seq_last_error().decode())
         segments = torch.empty(n // 4, dtype=torch.float32, device=u.device)
-        a.segments = segments.data_ptr()
-    _call("auv_selective_scan", a, _lib.SEQ_FORWARD, u.device)
-    return y, new_state, segments
+    block = _pack_scan(*head, _ptr(new), *_rows(y), _ptr(segments), *(0,) * 25)
+    _call("auv_selective_scan", block, _lib.SEQ_FORWARD, head[0])
+    return y, new, segments
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, softplus, return_state):
+    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, head, return_state, mark):
         ctx.set_materialize_grads(False)
-        y, new_state, segments = _scan_forward(u, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, softplus,
-                                               return_state, True)
+        y, new, segments = _scan_forward(u, A, state, head, return_state, True)
         ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, segments)
-        ctx.softplus = softplus
-        return y, new_state
+        ctx.softplus, ctx.mark = head[7], mark
+        return y, new
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dnew):
         u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, segments = ctx.saved_tensors
         want = ctx.needs_input_grad
+        rest = (None,) * 5
         if u.numel() == 0:
             out = [torch.zeros_like(t) if w else None
                    for t, w in zip((u, delta, A, Bm, Cm, D, z, delta_bias, state), want)]
             if want[8] and dnew is not None:
                 out[8] = dnew.clone()
-            return (*out, None, None, None, None)
+            return (*out, *rest)
         dy = torch.zeros_like(u) if dy is None else _adjacent(dy)
         dnew = None if dnew is None else dnew.contiguous()
-        a = _scan_args(u, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, ctx.softplus)
-        du, ddelta, dB, dC = (torch.empty_like(t) for t in (u, delta, Bm, Cm))
+        du, ddelta, dB, dC = torch.empty_like(u), torch.empty_like(delta), torch.empty_like(Bm), torch.empty_like(Cm)
         dz = None if z is None else torch.empty_like(z)
-        dA, dD, dbias, dstate = (torch.empty_like(t) if w else None
-                                 for t, w in ((A, want[2]), (D, want[5]), (delta_bias, want[7]), (state, want[8])))
-        for name, t, dims in (("d_y", dy, (0, 1)), ("d_u", du, (0, 1)), ("d_delta", ddelta, (0, 1)), ("d_z", dz, (0, 1)),
-                              ("d_B", dB, (0, 1, 2)), ("d_C", dC, (0, 1, 2))):
-            for k, v in _strides(name, t, *dims).items():
-                setattr(a, k, v)
-        a.segments, a.d_new_state = segments.data_ptr(), _ptr(dnew)
-        a.d_A, a.d_D, a.d_delta_bias, a.d_state = _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dstate)
-        _call("auv_selective_scan", a, _lib.SEQ_BACKWARD, u.device)
-        first = [g if w else None for g, w in zip((du, ddelta, dA, dB, dC, dD, dz, dbias, dstate), want)]
-        return (*first, None, None, None, None)
+        dA = torch.empty_like(A) if want[2] else None
+        dD = torch.empty_like(D) if want[5] else None
+        dbias = torch.empty_like(delta_bias) if want[7] else None
+        dstate = torch.empty_like(state) if want[8] else None
+        dev = u.get_device()
+        block = _pack_scan(dev, TYPES[u.dtype], *u.shape, A.shape[1], Bm.shape[2], ctx.softplus, *_rows(u), *_rows(delta), *_rows(z),
+                           *_groups(Bm), *_groups(Cm), A.data_ptr(), _ptr(D), _ptr(delta_bias), *_rows(start), _ptr(lengths), _ptr(state),
+                           0, 0, 0, 0, segments.data_ptr(), *_rows(dy), _ptr(dnew), *_rows(du), *_rows(ddelta), *_rows(dz),
+                           *_groups(dB), *_groups(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dstate))
+        _call("auv_selective_scan", block, _lib.SEQ_BACKWARD, dev)
+        return (*(g if w else None for g, w in zip((du, ddelta, dA, dB, dC, dD, dz, dbias, dstate), want)), *rest)
 
 
-def _check_scan(u, delta, A, Bm, Cm, D, z, delta_bias):
-    lead, Dc = tuple(u.shape[:-1]), u.shape[-1]
+def _scan_head(u, shape, u_strides, dev, delta, A, Bm, Cm, D, z, delta_bias, start, lengths, state, softplus, state_needed):
+    """The argument block up to state, in order, for rollouts [batch, length, channels] and for steps [batch, channels]."""
+    lead, Dc, dtype = shape[:-1], shape[-1], u.dtype
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
         raise ValueError(f"A must be [channels, states] with 1 to {MAX_STATES} states")
-    _dense("A", A, (Dc, A.shape[1]), u)
-    _activation("delta", delta, tuple(u.shape), u)
-    if z is not None:
-        _activation("z", z, tuple(u.shape), u)
-    if not isinstance(Bm, torch.Tensor) or Bm.dim() != u.dim() + 1 or Bm.shape[-2] < 1 or Dc % Bm.shape[-2]:
+    N = A.shape[1]
+    a = _dense("A", A, (Dc, N), dev)
+    ds = _like("delta", delta, shape, dtype, dev)
+    zs = None if z is None else _like("z", z, shape, dtype, dev)
+    if not isinstance(Bm, torch.Tensor) or Bm.dim() != len(shape) + 1 or Bm.shape[-2] < 1 or Dc % Bm.shape[-2]:
         raise ValueError("B must be [..., groups, states] with a number of groups that divides the channels")
-    shape = lead + (Bm.shape[-2], A.shape[1])
-    _activation("B", Bm, shape, u)
-    _activation("C", Cm, shape, u)
-    _dense("D", D, (Dc,), u)
-    _dense("delta_bias", delta_bias, (Dc,), u)
+    G = Bm.shape[-2]
+    bs = _like("B", Bm, lead + (G, N), dtype, dev)
+    cs = _like("C", Cm, lead + (G, N), dtype, dev)
+    skip, bias = _dense("D", D, (Dc,), dev), _dense("delta_bias", delta_bias, (Dc,), dev)
+    marks = _marks(start, lead, dev)
+    n = _dense("lengths", lengths, lead[:1], dev, torch.int32)
+    if state is None and state_needed:
+        raise TypeError("state must be a tensor, got None")
+    h = _dense("state", state, (lead[0], Dc, N), dev)
+    if len(lead) == 2:
+        row = lambda p, s: (p, s[0], s[1])            # noqa: E731
+        group = lambda p, s: (p, s[0], s[1], s[2])    # noqa: E731
+    else:
+        row = lambda p, s: (p, s[0], 0)               # noqa: E731
+        group = lambda p, s: (p, s[0], 0, s[1])       # noqa: E731
+    return (dev, TYPES[dtype], lead[0], lead[1] if len(lead) == 2 else 1, Dc, N, G, 1 if softplus else 0,
+            *row(u.data_ptr(), u_strides), *row(delta.data_ptr(), ds), *(row(z.data_ptr(), zs) if zs else (0, 0, 0)),
+            *group(Bm.data_ptr(), bs), *group(Cm.data_ptr(), cs), a, skip, bias, *marks, n, h)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, start=None, lengths=None,
@@ -392,19 +427,13 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_
     which `selective_scan_step` goes on from.  Differentiable in every float argument; for
     the backward pass the states before every 16th token are kept, N/4 bytes per element of u
     (N rounded up to 4, 8, 16, 32 or 64)."""
-    _activation("u", u)
-    if u.dim() != 3:
-        raise ValueError(f"u must be [batch, length, channels], got {tuple(u.shape)}")
-    _check_scan(u, delta, A, B, C, D, z, delta_bias)
-    _marks("start", start, tuple(u.shape[:2]), u)
-    _dense("lengths", lengths, (u.shape[0],), u, torch.int32)
-    _dense("state", state, (u.shape[0],) + tuple(A.shape), u)
+    shape, strides, dev = _first("u", u, 3, "[batch, length, channels]")
+    head = _scan_head(u, shape, strides, dev, delta, A, B, C, D, z, delta_bias, start, lengths, state, delta_softplus, False)
     tensors = (u, delta, A, B, C, D, z, delta_bias, state)
-    if _wants_grad(*tensors):
-        held = _guard_capture(*tensors)   # noqa: F841
-        y, new = _Scan.apply(*tensors, start, lengths, bool(delta_softplus), bool(return_state))
+    if _wants_grad(tensors):
+        y, new = _Scan.apply(*tensors, start, lengths, head, bool(return_state), _mark_graph(tensors))
     else:
-        y, new, _ = _scan_forward(*tensors[:8], start, lengths, state, delta_softplus, return_state, False)
+        y, new, _ = _scan_forward(u, A, state, head, return_state, False)
     return (y, new) if return_state else y
 
 
@@ -412,37 +441,18 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
                         new_state=None):
     """`selective_scan` of one token per row: u, delta, z [batch, channels]; B, C [batch, groups, N];
     `state` [batch, channels, N] moves on by the token, in place or into `new_state`."""
-    _activation("u", u)
-    if u.dim() != 2:
-        raise ValueError(f"u must be [batch, channels], got {tuple(u.shape)}")
-    _check_scan(u, delta, A, B, C, D, z, delta_bias)
-    if state is None:
-        raise TypeError("state must be a tensor, got None")
-    Bn, Dc = u.shape
-    shape = (Bn,) + tuple(A.shape)
-    _dense("state", state, shape, u)
-    _marks("start", start, (Bn,), u)
-    _no_grad_here("selective_scan_step", u, delta, state, A, B, C, D, z, delta_bias)
-    if new_state is None:
-        new_state = state
-    elif new_state is not state:
-        _dense("new_state", new_state, shape, u)
-        _written("new_state", new_state, ("state", state), ("A", A))
-    y = torch.empty((Bn, Dc), dtype=u.dtype, device=u.device)
-    if u.numel() == 0:
-        return y
-    row = lambda t: t.stride(0) if Bn > 1 else 0   # noqa: E731
-    group = lambda t: t.stride(1) if t.shape[1] > 1 else 0   # noqa: E731
-    a = _lib.AuvScanArgs(device=u.device.index, dtype=TYPES[u.dtype], batch=Bn, length=1, channels=Dc, states=A.shape[1],
-                         groups=B.shape[1], softplus=bool(delta_softplus), u=u.data_ptr(), u_row=row(u), delta=delta.data_ptr(),
-                         delta_row=row(delta), B=B.data_ptr(), B_row=row(B), B_group=group(B), C=C.data_ptr(), C_row=row(C),
-                         C_group=group(C), A=A.data_ptr(), D=_ptr(D), delta_bias=_ptr(delta_bias), state=state.data_ptr(),
-                         new_state=new_state.data_ptr(), y=y.data_ptr(), y_row=Dc)
-    if z is not None:
-        a.z, a.z_row = z.data_ptr(), row(z)
-    if start is not None:
-        a.start, a.start_row = start.data_ptr(), row(start)
-    _call("auv_selective_scan", a, _lib.SEQ_STEP, u.device)
+    shape, strides, dev = _first("u", u, 2, "[batch, channels]")
+    head = _scan_head(u, shape, strides, dev, delta, A, B, C, D, z, delta_bias, start, None, state, delta_softplus, True)
+    _no_grad_here("selective_scan_step", (u, delta, state, A, B, C, D, z, delta_bias))
+    to = head[-1]
+    if new_state is not None and new_state is not state:
+        to = _dense("new_state", new_state, state.shape, dev)
+        _apart("new_state", new_state, "state", state)
+        _apart("new_state", new_state, "A", A)
+    y = torch.empty(shape, dtype=u.dtype, device=u.device)
+    if shape[0] and shape[1]:
+        block = _pack_scan(*head, to, y.data_ptr(), shape[1], 0, *(0,) * 26)
+        _call("auv_selective_scan", block, _lib.SEQ_STEP, dev, scratch=False)
     return y
 
 
@@ -453,62 +463,56 @@ def _as_rows(t):
     """[..., channels] as [rows or batch, length, channels], without a copy where the strides allow one."""
     if t is None or t.dim() == 3:
         return t
-    return t.reshape(1, -1, t.shape[-1]) if t.dim() != 2 else t[None]
+    return t[None] if t.dim() == 2 else t.reshape(1, -1, t.shape[-1])
 
 
-def _norm_args(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
-    B, L, D = x.shape
-    return _lib.AuvNormArgs(device=x.device.index, dtype=TYPES[dtype], residual_dtype=TYPES[x.dtype], batch=B, length=L, channels=D,
-                            gate_act=GATES[gate_act], eps=eps, post_weight=_ptr(post_weight), pre_weight=_ptr(pre_weight),
-                            scale=_ptr(scale), **_strides("x", x, 0, 1), **_strides("y", y, 0, 1), **_strides("gate", gate, 0, 1))
+def _norm_head(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
+    """The argument block up to scale."""
+    return (x.get_device(), TYPES[dtype], TYPES[x.dtype], *x.shape, act, eps, *_rows(x), *_rows(y), *_rows(gate), _ptr(post_weight),
+            _ptr(pre_weight), _ptr(scale))
 
 
-def _norm_forward(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
+def _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
     out = torch.empty_like(x) if y is not None else None
-    h = None
-    if pre_weight is not None:
-        h = torch.empty_like(x if y is None else y, dtype=dtype)
+    h = torch.empty_like(x if y is None else y, dtype=dtype) if pre_weight is not None else None
     if x.numel():
-        a = _norm_args(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype)
-        for name, t in (("x_out", out), ("h", h)):
-            for k, v in _strides(name, t, 0, 1).items():
-                setattr(a, k, v)
-        _call("auv_residual_norm", a, _lib.SEQ_FORWARD, x.device)
+        head = _norm_head(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
+        _call("auv_residual_norm", _pack_norm(*head, *_rows(out), *_rows(h), *(0,) * 18), _lib.SEQ_FORWARD, head[0], scratch=False)
     return out, h
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
+    def forward(ctx, x, y, post_weight, pre_weight, gate, scale, act, eps, dtype, mark):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, post_weight, pre_weight, gate, scale)
-        ctx.how = (gate_act, eps, dtype)
-        return _norm_forward(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype)
+        ctx.how, ctx.mark = (act, eps, dtype), mark
+        return _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, d_h):
         x, y, post_weight, pre_weight, gate, scale = ctx.saved_tensors
         want = ctx.needs_input_grad
-        none = (None, None, None)
+        rest = (None,) * 4
         if d_out is None and d_h is None or x.numel() == 0:
             return tuple(torch.zeros_like(t) if w else None
-                         for t, w in zip((x, y, post_weight, pre_weight, gate, scale), want)) + none
+                         for t, w in zip((x, y, post_weight, pre_weight, gate, scale), want)) + rest
         d_out, d_h = _adjacent(d_out), _adjacent(d_h)
         dx = torch.empty_like(x)
-        dy, dgate = (None if t is None else torch.empty_like(t) for t in (y, gate))
-        dpost, dpre, dscale = (torch.empty_like(t) if w else None
-                               for t, w in ((post_weight, want[2]), (pre_weight, want[3]), (scale, want[5])))
-        a = _norm_args(x, y, post_weight, pre_weight, gate, scale, *ctx.how)
-        for name, t in (("d_x_out", d_out), ("d_h", d_h), ("d_x", dx), ("d_y", dy), ("d_gate", dgate)):
-            for k, v in _strides(name, t, 0, 1).items():
-                setattr(a, k, v)
-        a.d_post_weight, a.d_pre_weight, a.d_scale = _ptr(dpost), _ptr(dpre), _ptr(dscale)
-        _call("auv_residual_norm", a, _lib.SEQ_BACKWARD, x.device)
-        return tuple(g if w else None for g, w in zip((dx, dy, dpost, dpre, dgate, dscale), want)) + none
+        dy = None if y is None else torch.empty_like(y)
+        dgate = None if gate is None else torch.empty_like(gate)
+        dpost = torch.empty_like(post_weight) if want[2] else None
+        dpre = torch.empty_like(pre_weight) if want[3] else None
+        dscale = torch.empty_like(scale) if want[5] else None
+        head = _norm_head(x, y, post_weight, pre_weight, gate, scale, *ctx.how)
+        block = _pack_norm(*head, 0, 0, 0, 0, 0, 0, *_rows(d_out), *_rows(d_h), *_rows(dx), *_rows(dy), *_rows(dgate),
+                           _ptr(dpost), _ptr(dpre), _ptr(dscale))
+        _call("auv_residual_norm", block, _lib.SEQ_BACKWARD, head[0])
+        return tuple(g if w else None for g, w in zip((dx, dy, dpost, dpre, dgate, dscale), want)) + rest
 
 
-def _norm(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
+def _norm(x, dev, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
     D = x.shape[-1]
     if D < 1 or D > _lib.NORM_MAX_CHANNELS:
         raise ValueError(f"1 to {_lib.NORM_MAX_CHANNELS} channels, got {D}")
@@ -516,30 +520,33 @@ def _norm(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype):
         raise ValueError("eps must be positive")
     if gate_act not in GATES:
         raise ValueError(f"gate_act must be one of {tuple(GATES)}, got {gate_act!r}")
-    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("scale", scale)):
-        _dense(name, t, (D,), x)
-    shape = x.shape
-    xs, ys, gs = _as_rows(x), _as_rows(y), _as_rows(gate)
-    args = (xs, ys, post_weight, pre_weight, gs, scale)
-    if _wants_grad(x, y, post_weight, pre_weight, gate, scale):
-        held = _guard_capture(x, y, post_weight, pre_weight, gate, scale)   # noqa: F841
-        out, h = _Norm.apply(*args, gate_act, float(eps), dtype)
+    _dense("post_weight", post_weight, (D,), dev)
+    _dense("pre_weight", pre_weight, (D,), dev)
+    _dense("scale", scale, (D,), dev)
+    shape, act, eps = x.shape, GATES[gate_act], float(eps)
+    tensors = (x, y, post_weight, pre_weight, gate, scale)
+    if len(shape) != 3:
+        x, y, gate = _as_rows(x), _as_rows(y), _as_rows(gate)
+    if _wants_grad(tensors):
+        out, h = _Norm.apply(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype, _mark_graph(tensors))
     else:
-        out, h = _norm_forward(*args, gate_act, float(eps), dtype)
-    return tuple(t if t is None else t.reshape(shape) for t in (out, h))
+        out, h = _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
+    if len(shape) != 3:
+        out, h = (t if t is None else t.reshape(shape) for t in (out, h))
+    return out, h
 
 
 def rms_norm(x, weight, *, eps=1e-6, dtype=None):
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension, x [..., channels] (at most 8,192),
     as `dtype` (x's own by default; float32 x may give bfloat16 or float16): the norm before a
     first block.  Differentiable in x and weight."""
-    _activation("x", x)
-    if x.dim() < 1 or weight is None:
-        raise ValueError("x must have a channel dimension and weight be given")
+    _, _, dev = _first("x", x, None, None)
+    if weight is None:
+        raise TypeError("weight must be a tensor, got None")
     dtype = x.dtype if dtype is None else dtype
     if dtype not in TYPES or (x.dtype != torch.float32 and x.dtype != dtype):
         raise TypeError(f"a norm of {x.dtype} cannot be {dtype}")
-    return _norm(x, None, None, weight, None, None, None, eps, dtype)[1]
+    return _norm(x, dev, None, None, weight, None, None, None, eps, dtype)[1]
 
 
 def residual_norm(x, y, post_weight=None, pre_weight=None, gate=None, scale=None, *, gate_act="silu", eps=1e-6):
@@ -554,17 +561,15 @@ def residual_norm(x, y, post_weight=None, pre_weight=None, gate=None, scale=None
     and scale are float32 [channels]; gate_act is "silu", "sigmoid" or None.  A gate that is the
     same for several tokens is given expanded (`gate.expand_as(y)`).  Differentiable in every
     float argument."""
-    _activation("x", x)
-    _activation("y", y, tuple(x.shape))
-    if y.device != x.device:
-        raise ValueError(f"y is on {y.device}, x on {x.device}")
-    if x.dtype not in (torch.float32, y.dtype):
-        raise TypeError(f"x must be float32 or y's {y.dtype}, got {x.dtype}")
-    if x.dim() < 1:
-        raise ValueError("x must have a channel dimension")
+    shape, _, dev = _first("x", x, None, None)
+    if not isinstance(y, torch.Tensor):
+        raise TypeError(f"y must be a tensor, got {type(y).__name__}")
+    if y.dtype not in TYPES or x.dtype not in (torch.float32, y.dtype):
+        raise TypeError(f"x must be float32 or of y's type, got {x.dtype} and {y.dtype}")
+    _like("y", y, shape, y.dtype, dev)
     if gate is not None:
-        _activation("gate", gate, tuple(x.shape), y)
-    return _norm(x, y, post_weight, pre_weight, gate, scale, gate_act, eps, y.dtype)
+        _like("gate", gate, shape, y.dtype, dev)
+    return _norm(x, dev, y, post_weight, pre_weight, gate, scale, gate_act, eps, y.dtype)
 
 
 # ----------------------------------------------------------------------------
