@@ -67,32 +67,36 @@ __device__ __forceinline__ float step_slope(float raw, int softplus) { return so
 
 // ----------------------------------------------------------------------------------------------------------------
 // Forward.  S lanes per channel, NPL states per lane: 64 / S channels per wave, a wave per (channel tile, group, row,
-// chunk of time).  B and C of the next tokens go through LDS once per wave as floats, zero-padded to NP states, which
+// chunk of time).  With S > 1 the lanes of a channel share the element-wise work of its tokens.  B and C of the next tokens go through LDS once per wave as floats, zero-padded to NP states, which
 // takes care of odd counts and strides; every lane of a channel reads them from there at the same address.
 //
 // MODE 0 computes outputs (from `state`, or from the chunk's entry state when the row is split into chunks).
 // MODE 1 starts each chunk from zero and leaves only its end state and its decay, exp(A sum dt) (0 behind a start).
 // ----------------------------------------------------------------------------------------------------------------
-constexpr int kScanTile = 8;
 template <int S>
 constexpr int lane_bits() { return S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0; }
+template <int S>
+// Tokens at a time: at least one for every lane of a channel.  Four where a lane has whole channels: eight take 233
+// registers (two waves per SIMD, 398 us for 4,096 x 128 x 128 in bf16 with 16 states), four 165 (three, 356 us).
+constexpr int scan_tile() { return S > 8 ? S : S == 1 ? 4 : 8; }
 
 template <class T, int NPL, int S, int MODE>
 __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
-    constexpr int NP = NPL * S, CW = 64 / S, TQ = kScanTile, SB = lane_bits<S>();
+    constexpr int NP = NPL * S, CW = 64 / S, TQ = scan_tile<S>(), KT = TQ / S, SB = lane_bits<S>();
     constexpr int BE = (TQ * NP + 63) / 64;   // elements of B (and of C) a lane carries into LDS per tile
     __shared__ __align__(16) float tile[kScanWaves][TQ][2][NP];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int q = lane % S, c = lane / S;
-    const int64_t Dg = a.D / a.G, tiles = (Dg + CW - 1) / CW;
-    int64_t id = (int64_t)blockIdx.x * kScanWaves + wave;
-    const int64_t ct = id % tiles;
+    const int Dg = (int)(a.D / a.G), tiles = (Dg + CW - 1) / CW;
+    unsigned id = blockIdx.x * kScanWaves + wave;             // the host sees to it that there are fewer than 2^31
+    const int ct = id % tiles;
     id /= tiles;
-    const int64_t g = id % a.G;
-    id /= a.G;
-    const int64_t b = id % a.B, chunk = id / a.B;
+    const int g = id % (unsigned)a.G;
+    id /= (unsigned)a.G;
+    const unsigned chunk = id / (unsigned)a.B, b32 = id - chunk * (unsigned)a.B;
     if (chunk >= a.chunks) return;
-    const int d_first = (int)(g * Dg + ct * CW), d_left = (int)(Dg - ct * CW);
+    const int64_t b = b32;
+    const int d_first = g * Dg + ct * CW, d_left = Dg - ct * CW;
     const bool live = c < d_left;
     const int dl = live ? c : d_left - 1;      // channel within the wave's tile
     const int64_t d = d_first + dl;
@@ -112,29 +116,32 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
         }
     }
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dv ? a.Dv[d] : 0.0f;
-    // the wave's place in each array is a scalar; a lane adds its channel
+    // the wave's place in each array is a scalar; a lane adds its channel and its first token
     const T* const u = (const T*)a.u + b * a.u_row + d_first;
     const T* const delta = (const T*)a.delta + b * a.delta_row + d_first;
     const T* const z = (const T*)a.z + b * a.z_row + d_first;
     const T* const Bm = (const T*)a.Bm + b * a.B_row + g * a.B_group;
     const T* const Cm = (const T*)a.Cm + b * a.C_row + g * a.C_group;
     T* const y = (T*)a.y + b * a.y_row + d_first;
+    const int64_t u_lane = q * a.u_token + dl, delta_lane = q * a.delta_token + dl, z_lane = q * a.z_token + dl, y_lane = q * a.y_token + dl;
     float sum_dt = 0.0f;
     bool cut = false;
 
-    // what a tile needs from memory, fetched one tile ahead
-    T ru[TQ], rd[TQ], rz[TQ], rB[BE], rC[BE];
+    // What a tile needs from memory, fetched one tile ahead.  The lanes of a channel take a token each, form its width and
+    // its gate, and hand them round.
+    T ru[KT], rd[KT], rz[KT], rB[BE], rC[BE];
     uint8_t mark = 0;
-    auto fetch = [&](int64_t t0) {
+    auto ask = [&](int64_t t0) {
         if (t0 >= stop) return;
         const int left = stop - t0 < TQ ? (int)(stop - t0) : TQ;
 #pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            const int64_t t = t0 + (i < left ? i : left - 1);
-            ru[i] = (u + t * a.u_token)[dl];
-            rd[i] = (delta + t * a.delta_token)[dl];
-            if (MODE == 0 && a.z) rz[i] = (z + t * a.z_token)[dl];
-        }
+        for (int k = 0; k < KT; ++k)
+            if (k * S + q < left) {
+                const int64_t t = t0 + k * S;
+                ru[k] = (u + t * a.u_token)[u_lane];
+                rd[k] = (delta + t * a.delta_token)[delta_lane];
+                if (MODE == 0 && a.z) rz[k] = (z + t * a.z_token)[z_lane];
+            }
 #pragma unroll
         for (int k = 0; k < BE; ++k) {
             const int e = k * 64 + lane, i = e / NP, s = e % NP;
@@ -145,7 +152,9 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
         mark = 0;
         if (a.start && lane < left) mark = a.start[b * a.start_row + (t0 + lane) * a.start_token];
     };
-    fetch(t_begin);
+#pragma unroll
+    for (int k = 0; k < KT; ++k) ru[k] = rd[k] = rz[k] = (T)0.0f;
+    ask(t_begin);
     for (int64_t t0 = t_begin; t0 < stop; t0 += TQ) {
         const int left = stop - t0 < TQ ? (int)(stop - t0) : TQ;
         if (MODE == 0 && a.segments && t0 % kSegment == 0 && live) {
@@ -154,16 +163,18 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
             for (int j = 0; j < NPL; j += 4) *reinterpret_cast<float4*>(seg + j) = make_float4(h[j], h[j + 1], h[j + 2], h[j + 3]);
         }
         const unsigned long long marks = __ballot(mark != 0);
-        float uu[TQ], dt[TQ], sz[TQ];
+        float uu[KT], dt[KT], du[KT], sz[KT];
 #pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            uu[i] = (float)ru[i];
-            dt[i] = step_width((float)rd[i] + bias, a.softplus);
-            sz[i] = 1.0f;
+        for (int k = 0; k < KT; ++k) {
+            uu[k] = (float)ru[k];
+            dt[k] = step_width((float)rd[k] + bias, a.softplus);
+            du[k] = dt[k] * uu[k];
+            sz[k] = 1.0f;
             if (MODE == 0 && a.z) {
-                const float zz = (float)rz[i];
-                sz[i] = zz * sigmoid_f(zz);
+                const float zz = (float)rz[k];
+                sz[k] = zz * sigmoid_f(zz);
             }
+            if (MODE == 1 && k * S + q < left) sum_dt += dt[k];
         }
         wave_sync();
 #pragma unroll
@@ -175,43 +186,53 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
             }
         }
         wave_sync();
-        fetch(t0 + TQ);
-        auto token = [&](int i) {
-            const float du = dt[i] * uu[i];
-            if (MODE == 1) sum_dt += dt[i];
-            float e[NPL], acc0 = 0.0f, acc1 = 0.0f;
+        ask(t0 + TQ);
+        auto tokens = [&](auto plain) {
+            constexpr bool PLAIN = decltype(plain)::value;      // a whole tile without a start in it
+            static_for<KT>([&](auto kk) {
+                constexpr int k = decltype(kk)::value;
+                float part[S];
+                static_for<S>([&](auto oo) {
+                    constexpr int o = decltype(oo)::value, i = k * S + o;
+                    part[o] = 0.0f;
+                    if (PLAIN || i < left) {
+                        if (!PLAIN && (marks >> i & 1)) {
+                            cut = true;
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) e[j] = exp2_hw(dt[i] * A2[j]);
+                            for (int j = 0; j < NPL; ++j) h[j] = 0.0f;
+                        }
+                        const float w = lane_spread<S, o>(dt[k]), x = lane_spread<S, o>(du[k]);
+                        float e[NPL], acc0, acc1;
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) h[j] = fmaf(e[j], h[j], du * tile[wave][i][0][q * NPL + j]);
-            if (MODE == 0) {
+                        for (int j = 0; j < NPL; ++j) e[j] = exp2_hw(w * A2[j]);
 #pragma unroll
-                for (int j = 0; j < NPL; j += 2) {
-                    acc0 = fmaf(h[j], tile[wave][i][1][q * NPL + j], acc0);
-                    acc1 = fmaf(h[j + 1], tile[wave][i][1][q * NPL + j + 1], acc1);
-                }
-                const float sum = lane_sum<SB>(acc0 + acc1);
-                if (live && q == 0) (y + (t0 + i) * a.y_token)[dl] = (T)(fmaf(skip, uu[i], sum) * sz[i]);
-            }
-        };
-        if (left == TQ && marks == 0) {
+                        for (int j = 0; j < NPL; ++j) h[j] = fmaf(e[j], h[j], x * tile[wave][i][0][q * NPL + j]);
+                        if (MODE == 0) {
+                            acc0 = h[0] * tile[wave][i][1][q * NPL];
+                            acc1 = h[1] * tile[wave][i][1][q * NPL + 1];
 #pragma unroll
-            for (int i = 0; i < TQ; ++i) token(i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < TQ; ++i) {
-                if (i < left) {
-                    if (marks >> i & 1) {
-                        cut = true;
-#pragma unroll
-                        for (int j = 0; j < NPL; ++j) h[j] = 0.0f;
+                            for (int j = 2; j < NPL; j += 2) {
+                                acc0 = fmaf(h[j], tile[wave][i][1][q * NPL + j], acc0);
+                                acc1 = fmaf(h[j + 1], tile[wave][i][1][q * NPL + j + 1], acc1);
+                            }
+                            part[o] = acc0 + acc1;
+                        }
+                        // sixteen states a token are enough to schedule among; more tokens at once cost registers, that is waves
+                        if (NPL >= 16) __builtin_amdgcn_sched_barrier(0);
                     }
-                    token(i);
+                });
+                if (MODE == 0) {
+                    lane_scatter_sum<SB, 0, S>(part);      // lane q gets the sum of token k S + q
+                    if (live && (PLAIN || k * S + q < left))
+                        (y + (t0 + k * S) * a.y_token)[y_lane] = (T)(fmaf(skip, uu[k], part[0]) * sz[k]);
                 }
-            }
-        }
+            });
+        };
+        if (left == TQ && marks == 0) tokens(std::true_type{});
+        else tokens(std::false_type{});
     }
     if (MODE == 1) {
+        sum_dt = lane_sum<SB>(sum_dt);     // over the tokens that a channel's lanes had
         if (live) {
             const int64_t o = ((chunk * a.B + b) * a.D + d) * NP + q * NPL;
 #pragma unroll

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 namespace auv {
 namespace seq {
@@ -134,6 +136,30 @@ __device__ __forceinline__ float dpp(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kQuadXor3 = 0x1b, kHalfMirror = 0x141, kMirror = 0x140, kRotate8 = 0x128;
+
+// f(0), f(1), ... f(N - 1) with the number as a compile-time constant.
+template <class F, int... I>
+__device__ __forceinline__ void static_for_(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_(f, std::make_integer_sequence<int, N>{});
+}
+
+// What lane FROM of every group of S adjacent lanes holds, in all of the group.
+template <int S, int FROM>
+__device__ __forceinline__ float lane_spread(float x) {
+    static_assert(FROM < S, "a lane of the group");
+    if constexpr (S == 1) return x;
+    else if constexpr (S == 2) return dpp<FROM ? 0xf5 : 0xa0>(x);
+    else if constexpr (S == 4) return dpp<FROM * 0x55>(x);
+    else if constexpr (S == 16) return dpp<0x150 + FROM>(x);
+    else {
+        const float low = dpp<0x150 + FROM>(x), high = dpp<0x158 + FROM>(x);
+        return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) & 8 ? high : low;
+    }
+}
 
 // After this, a holds both registers' low (BIT clear) parts side by side and b both high parts.
 template <int BIT>
