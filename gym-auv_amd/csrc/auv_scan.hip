@@ -173,18 +173,13 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
 }
 
 template <class T, int S>
-int run_step(const ScanArgs& a, hipStream_t stream) {
-    Width whole(4);
-    whole.pointer(a.Bm, sizeof(T));
-    whole.pointer(a.Cm, sizeof(T));
-    if (a.B > 1) whole.stride(a.B_row), whole.stride(a.C_row);
-    if (a.G > 1) whole.stride(a.B_group), whole.stride(a.C_group);
-    for (const float* q : {a.A, a.state, (const float*)a.new_state}) whole.pointer(q, 4);
-    const dim3 grid((unsigned)ceil_div(a.B * a.D * S, 256)), block(256);
-    if (a.N == 4 * S && whole.elements() == 4)
-        hipLaunchKernelGGL((k_scan_step<T, S, true>), grid, block, 0, stream, a);
-    else
-        hipLaunchKernelGGL((k_scan_step<T, S, false>), grid, block, 0, stream, a);
+int run_step(ScanArgs a, hipStream_t stream) {
+    const int64_t lanes = a.D * S < kStepThreads ? a.D * S : kStepThreads, tiles = ceil_div(a.D * S, lanes);
+    a.lanes = (int32_t)lanes;
+    // eight workgroups per CU, each with as many rows as it takes
+    const int64_t want = ceil_div(a.B, kStepThreads / lanes), most = ceil_div(2048, tiles);
+    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)tiles), block(kStepThreads);
+    hipLaunchKernelGGL((k_scan_step<T, S>), grid, block, 0, stream, a);
     return launched("k_scan_step");
 }
 
@@ -249,15 +244,16 @@ int64_t workspace(const auv_scan_args& p, int32_t pass) {
 
 int launches_fit(const auv_scan_args& p, int32_t pass) {
     const int S = lanes_of(p.states);
-    int64_t most = 0;
-    if (pass == AUV_SEQ_STEP) most = ceil_div(p.batch * p.channels * S, 256);
+    // (states of 4 TiB would not fit the device either)
+    int64_t most = p.batch * p.channels > ((int64_t)1 << 40) / p.states ? kMaxGrid + 1 : 0;
+    if (pass == AUV_SEQ_STEP && ceil_div(p.channels * S, kStepThreads) > 65535) return seq_fail(AUV_ERR_ARG, "auv_selective_scan: too many channels");
     if (pass == AUV_SEQ_FORWARD) {
         const Forward f = forward_plan(p);
-        most = f.waves * f.chunks.count;   // numbered in 32 bits
+        if (f.waves * f.chunks.count > kMaxGrid) most = kMaxGrid + 1;   // numbered in 32 bits
     }
     if (pass == AUV_SEQ_BACKWARD) {
         const Backward r = backward_plan(p);
-        most = r.bc_bytes ? ceil_div(p.batch * p.length * p.groups * 8 * S, 256) : 0;
+        if (r.bc_bytes && ceil_div(p.batch * p.length * p.groups * 8 * S, 256) > kMaxGrid) most = kMaxGrid + 1;
     }
     return most > kMaxGrid ? seq_fail(AUV_ERR_ARG, "auv_selective_scan: batch too large for one launch") : AUV_OK;
 }

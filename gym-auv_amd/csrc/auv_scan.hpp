@@ -51,6 +51,7 @@ struct ScanArgs {
     int64_t dB_row, dB_token, dB_group, dC_row, dC_token, dC_group;
     float* dstate;           // [B,D,N]
     float* partial;          // [gridDim.x * units per workgroup, D, N + 2]: dA, dD, ddelta_bias
+    int32_t lanes;           // threads side by side on a row's channels in a step
     int32_t whole;           // rows of activations and of their gradients may be read and written in fours
     float* bc_partial;       // [tile blocks, B, L, G, 2, NP] when a group's channels fill more than one workgroup
 };
@@ -771,62 +772,63 @@ __global__ __launch_bounds__(256) void k_scan_sum_bc(ScanArgs a, int NP, int blo
 
 // ----------------------------------------------------------------------------------------------------------------
 // One token per row: the states once in, once out, 8 N bytes per channel against some 50 bytes of everything else.  A
-// lane holds 4 states, S lanes a channel, so that a wave reads 1 KiB of adjacent states per load.  state and new_state
-// may be the same memory: a lane writes only what it alone has read.
+// lane holds 4 states, S lanes a channel, so that a wave reads 1 KiB of adjacent states per load; it keeps its channel's
+// parameters for all the rows it takes and asks for the next row's states while it works on one.  state and new_state may
+// be the same memory: a lane writes only what it alone has read.
 // ----------------------------------------------------------------------------------------------------------------
-template <class T, int S, bool WHOLE>   // WHOLE: N = 4 S and everything a lane loads in fours is aligned for it
-__global__ __launch_bounds__(256) void k_scan_step(ScanArgs a) {
+constexpr int kStepThreads = 256;
+template <class T, int S>
+__global__ __launch_bounds__(kStepThreads) void k_scan_step(ScanArgs a) {
     constexpr int SB = lane_bits<S>();
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S;   // (row, channel)
-    const int q = threadIdx.x % S;
-    const bool live = i < a.B * a.D;
-    const int64_t b = live ? i / a.D : 0, d = live ? i - b * a.D : 0;
-    const int64_t g = d / (a.D / a.G);
-    float h[4], A[4], Bv[4], Cv[4];
-    const T* const Bm = (const T*)a.Bm + b * a.B_row + g * a.B_group + q * 4;
-    const T* const Cm = (const T*)a.Cm + b * a.C_row + g * a.C_group + q * 4;
-    const int64_t o = (b * a.D + d) * a.N + q * 4;
-    if (WHOLE) {
-        load<float, 4>(a.state + o, h);
-        load<float, 4>(a.A + d * a.N + q * 4, A);
-        load<T, 4>(Bm, Bv);
-        load<T, 4>(Cm, Cv);
-    } else {
+    // a.lanes threads (a multiple of S) take a row's channels, as many of them as there are or as a workgroup holds
+    const int lane = threadIdx.x % a.lanes, slot = threadIdx.x / a.lanes, slots = kStepThreads / a.lanes;
+    const int64_t d = (int64_t)blockIdx.y * (a.lanes / S) + lane / S;
+    const int q = lane % S;
+    if (slot >= slots || d >= a.D) return;      // all lanes of a channel or none
+    const int g = (int)(d / (a.D / a.G)), count = clamp_count(a.N - q * 4, 4);
+    float A2[4];
+    Raw<float, 4> rA;
+    fetch(rA, a.A + d * a.N + q * 4, count);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A2[j] = rA.at(j) * kLog2e;
+    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dv ? a.Dv[d] : 0.0f;
+    Raw<float, 4> rh = {};
+    Raw<T, 4> rB = {}, rC = {};
+    T ru = (T)0.0f, rd = (T)0.0f, rz = (T)0.0f;
+    uint8_t mark = 0;
+    auto ask = [&](int64_t b) {
+        if (b >= a.B) return;
+        fetch(rh, a.state + (b * a.D + d) * a.N + q * 4, count);
+        fetch(rB, (const T*)a.Bm + b * a.B_row + g * a.B_group + q * 4, count);
+        fetch(rC, (const T*)a.Cm + b * a.C_row + g * a.C_group + q * 4, count);
+        ru = ((const T*)a.u)[b * a.u_row + d];
+        rd = ((const T*)a.delta)[b * a.delta_row + d];
+        if (a.z) rz = ((const T*)a.z)[b * a.z_row + d];
+        if (a.start) mark = a.start[b * a.start_row];
+    };
+    const int64_t step = (int64_t)gridDim.x * slots;
+    int64_t b = (int64_t)blockIdx.x * slots + slot;
+    ask(b);
+    for (; b < a.B; b += step) {
+        float h[4], x[4], C[4];
+        const float u = (float)ru, z = (float)rz;
+        const float dt = step_width((float)rd + bias, a.softplus);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = mark ? 0.0f : rh.at(j), x[j] = dt * u * rB.at(j), C[j] = rC.at(j);
+        ask(b + step);
+        float acc = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool in = q * 4 + j < a.N;
-            h[j] = in ? a.state[o + j] : 0.0f;
-            A[j] = in ? a.A[d * a.N + q * 4 + j] : 0.0f;
-            Bv[j] = in ? (float)Bm[j] : 0.0f;
-            Cv[j] = in ? (float)Cm[j] : 0.0f;
+            h[j] = fmaf(exp2_hw(dt * A2[j]), h[j], x[j]);
+            acc = fmaf(h[j], C[j], acc);
         }
-    }
-    if (a.start && a.start[b * a.start_row]) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = 0.0f;
-    }
-    const float u = (float)((const T*)a.u)[b * a.u_row + d];
-    const float dt = step_width((float)((const T*)a.delta)[b * a.delta_row + d] + (a.bias ? a.bias[d] : 0.0f), a.softplus);
-    float acc = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        h[j] = fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[j], dt * u * Bv[j]);
-        acc = fmaf(h[j], Cv[j], acc);
-    }
-    acc = lane_sum<SB>(acc);
-    if (!live) return;
-    if (WHOLE) store<float, 4>(a.new_state + o, h);
-    else
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (q * 4 + j < a.N) a.new_state[o + j] = h[j];
-    if (q == 0) {
-        acc = fmaf(a.Dv ? a.Dv[d] : 0.0f, u, acc);
-        if (a.z) {
-            const float z = (float)((const T*)a.z)[b * a.z_row + d];
-            acc *= z * sigmoid_f(z);
+        acc = lane_sum<SB>(acc);
+        put(a.new_state + (b * a.D + d) * a.N + q * 4, count, h);
+        if (q == 0) {
+            acc = fmaf(skip, u, acc);
+            if (a.z) acc *= z * sigmoid_f(z);
+            ((T*)a.y)[b * a.y_row + d] = (T)acc;
         }
-        ((T*)a.y)[b * a.y_row + d] = (T)acc;
     }
 }
 
