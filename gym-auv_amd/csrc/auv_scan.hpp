@@ -389,6 +389,9 @@ __device__ __forceinline__ int thread_anew() {
     return t;
 }
 
+// i times a stride, of two instructions
+__device__ __forceinline__ int64_t times(int i, int64_t stride) { return (int64_t)((uint64_t)(unsigned)i * (uint64_t)stride); }
+
 // MODE 0: gradients.  MODE 1: from zero at the end of each chunk, only the carry at its front and its decay.
 template <class T, int S, int MODE>
 __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 : 2) void k_scan_backward(ScanArgs a) {
@@ -511,12 +514,15 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
             for (int k = 0; k < BE; ++k) {
                 const int e = tid + k * TH;
                 if (k * TH < units * Q * 2 * NP) {
-                    const int un = e / (Q * 2 * NP), i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
+                    // (rows of a workgroup's worth of numbers or more: the row is the same for all threads)
+                    const int un = TH <= Q * 2 * NP ? k * TH / (Q * 2 * NP) : e / (Q * 2 * NP);
+                    const int i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
                     fbc[k] = (T)0.0f;
                     if (un < units && s < N && t0 + i < len[un]) {
-                        const int64_t br = row0 + un;
-                        if (which == 1) fbc[k] = ((const T*)r.Cm + br * r.C_row + g * r.C_group + t0 * r.C_token)[i * r.C_token + s];
-                        else if (MODE == 0) fbc[k] = ((const T*)r.Bm + br * r.B_row + g * r.B_group + t0 * r.B_token)[i * r.B_token + s];
+                        if (which == 1)
+                            fbc[k] = ((const T*)r.Cm + (row0 + un) * r.C_row + g * r.C_group + t0 * r.C_token)[times(i, r.C_token) + s];
+                        else if (MODE == 0)
+                            fbc[k] = ((const T*)r.Bm + (row0 + un) * r.B_row + g * r.B_group + t0 * r.B_token)[times(i, r.B_token) + s];
                     }
                 }
             }
@@ -704,18 +710,21 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
                 store<float, 4>(sums[threadIdx.x], dD);
                 store<float, 4>(sums[TH + threadIdx.x], dbias);
             }
-            for (int e = thread_anew(); e < units * Q * 2 * NP; e += TH) {
-                const int un = e / (Q * 2 * NP), i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
-                const int64_t br = row0 + un, t = t0 + i;
-                if (br < r.B && t < t_end && s < N) {
+            const int me_again = thread_anew();
+            for (int k = 0; k * TH < units * Q * 2 * NP; ++k) {
+                const int e = me_again + k * TH;
+                const int un = TH <= Q * 2 * NP ? k * TH / (Q * 2 * NP) : e / (Q * 2 * NP);
+                const int i = e / (2 * NP) % Q, which = e / NP % 2, s = e % NP;
+                if (un < units && row0 + un < r.B && t0 + i < t_end && s < N) {
+                    const int64_t br = row0 + un;
                     float sum = 0.0f;
                     for (int w = 0; w < per; ++w) sum += red[((un * per + w) * Q + i) * 2 * NP + which * NP + s];
                     if (r.bc_partial)
-                        r.bc_partial[((((int64_t)tb * r.B + br) * r.L + t) * r.G + g) * 2 * NP + which * NP + s] = sum;
+                        (r.bc_partial + (((int64_t)tb * r.B + br) * r.L + t0) * r.G * 2 * NP)[times(i, r.G * 2 * NP) + (g * 2 + which) * NP + s] = sum;
                     else if (which == 0)
-                        ((T*)r.dB + br * r.dB_row + t * r.dB_token + g * r.dB_group)[s] = (T)sum;
+                        ((T*)r.dB + br * r.dB_row + t0 * r.dB_token + g * r.dB_group)[times(i, r.dB_token) + s] = (T)sum;
                     else
-                        ((T*)r.dC + br * r.dC_row + t * r.dC_token + g * r.dC_group)[s] = (T)sum;
+                        ((T*)r.dC + br * r.dC_row + t0 * r.dC_token + g * r.dC_group)[times(i, r.dC_token) + s] = (T)sum;
                 }
             }
         }

@@ -199,6 +199,10 @@ _pack_room = struct.Struct("<2q").pack
 _NO_ROOM = _pack_room(0, 0)
 
 
+# the current stream's handle without the Stream object round it, where this torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _call(name, block, what, dev, scratch=True):
     """Runs entry point `name` on the current stream, with the scratch memory it asks for."""
     lib = _lib.load()
@@ -210,7 +214,7 @@ def _call(name, block, what, dev, scratch=True):
         if room:
             held = torch.empty(room, dtype=torch.uint8, device=dev)   # the stream's own: free for it again on return
             tail = _pack_room(held.data_ptr(), room)
-    rc = getattr(lib, name)(block + tail, what, torch.cuda.current_stream(dev).cuda_stream)
+    rc = getattr(lib, name)(block + tail, what, _raw_stream(dev))
     if rc != 0:
         raise _lib.AuvError(rc, lib.auv_seq_last_error().decode())
 
