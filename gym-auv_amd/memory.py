@@ -128,6 +128,14 @@ def _apart(name, t, other_name, o):
         raise ValueError(f"{name} overlaps {other_name}")
 
 
+def _in_place(name, lo, t, others):
+    """A step's new state, t's worth of memory from address lo on, holds none of the step's inputs (by their addresses)."""
+    hi = lo + t.numel() * t.element_size()
+    for p in others:
+        if lo <= p < hi:
+            raise ValueError(f"{name} holds an input of the step")
+
+
 def _wants_grad(tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -157,6 +165,8 @@ def _mark_graph(tensors):
     runs those on the eager graph's stream, and joining that stream to a capture ends the process.  Returns what the
     call's own node is to keep."""
     leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
+    if not leaves:
+        return None
     if torch.cuda.is_current_stream_capturing():
         if any(leaves & g.leaves for g in list(_eager_graphs)):
             raise RuntimeError("a graph that records gradients is being captured while the outputs of an earlier eager pass "
@@ -316,7 +326,7 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, (B, W - 1, D), dev, x.dtype)
         _apart("new_state", new_state, "state", state)
-        _apart("new_state", new_state, "x", x)
+    _in_place("the new state", to, state, (x.data_ptr(), weight.data_ptr(), _ptr(bias), marks[0]))
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
     if B and D:
         block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
@@ -452,7 +462,7 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, state.shape, dev)
         _apart("new_state", new_state, "state", state)
-        _apart("new_state", new_state, "A", A)
+    _in_place("the new state", to, state, (head[8], head[11], head[14], head[17], head[21], *head[25:29]))
     y = torch.empty(shape, dtype=u.dtype, device=u.device)
     if shape[0] and shape[1]:
         block = _pack_scan(*head, to, y.data_ptr(), shape[1], 0, *(0,) * 26)
