@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kConvThreads) void k_conv_forward(ConvArgs a) {
 #pragma unroll
                         for (int v = 0; v < V; ++v) {
                             const float pre = conv_pre<W, V>(xs, w, bias, i, v);
-                            out[v] = a.silu ? pre * sigmoid_f(pre) : pre;
+                            out[v] = a.silu ? pre * sigmoid_f<T>(pre) : pre;
                         }
                         put(y, V, out);
                         y += a.y_token;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kConvThreads, 2) void k_conv_backward(ConvArgs a) {
                         for (int v = 0; v < V; ++v) {
                             float g = out[v];
                             if (a.silu) {
-                                const float pre = conv_pre<W, V>(xs, w, bias, i, v), s = sigmoid_f(pre);
+                                const float pre = conv_pre<W, V>(xs, w, bias, i, v), s = sigmoid_f<T>(pre);
                                 g *= s * fmaf(pre, 1.0f - s, 1.0f);
                             }
                             gs[i][v] = t < c.real ? g : 0.0f;
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kConvThreads) void k_conv_step(ConvArgs a) {
             float pre = bias[v];
 #pragma unroll
             for (int k = 0; k < W; ++k) pre = fmaf(win[k][v], w[v * W + k], pre);
-            out[v] = a.silu ? pre * sigmoid_f(pre) : pre;
+            out[v] = a.silu ? pre * sigmoid_f<T>(pre) : pre;
         }
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) put((T*)a.new_state + (b * (W - 1) + k) * a.D + d, count, win[k + 1]);

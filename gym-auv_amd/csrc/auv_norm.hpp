@@ -61,8 +61,9 @@ __device__ __forceinline__ void row_sum(float (&v)[NSUM], float (*buf)[NSUM]) {
     }
 }
 
+template <class T>
 __device__ __forceinline__ float gate_value(float g, int act) {
-    return act == 0 ? g : act == 1 ? g * sigmoid_f(g) : sigmoid_f(g);
+    return act == 0 ? g : act == 1 ? g * sigmoid_f<T>(g) : sigmoid_f<T>(g);
 }
 template <class TR, class T, int TPR>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
         for (int v = 0; v < V; ++v) {
             float n = ry.at(v);
             if (a.post_weight) n *= r1 * w.at(v);
-            if (a.gate) n *= gate_value(rg.at(v), a.act);
+            if (a.gate) n *= gate_value<T>(rg.at(v), a.act);
             if (a.scale) n *= s.at(v);
             r[v] += n;
         }
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
                 const float g = fg.at(v);
                 act[v] = g;
                 if (a.act != 0) {
-                    const float s = sigmoid_f(g);
+                    const float s = sigmoid_f<T>(g);
                     act[v] = a.act == 1 ? g * s : s;
                     slope[v] = a.act == 1 ? s * fmaf(g, 1.0f - s, 1.0f) : s * (1.0f - s);
                 }

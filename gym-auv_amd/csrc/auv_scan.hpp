@@ -63,8 +63,10 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // delta -> step width, and the width's derivative with respect to delta
-__device__ __forceinline__ float step_width(float raw, int softplus) { return softplus ? softplus_f(raw) : raw; }
-__device__ __forceinline__ float step_slope(float raw, int softplus) { return softplus ? sigmoid_f(raw) : 1.0f; }
+template <class T>
+__device__ __forceinline__ float step_width(float raw, int softplus) { return softplus ? softplus_f<T>(raw) : raw; }
+template <class T>
+__device__ __forceinline__ float step_slope(float raw, int softplus) { return softplus ? sigmoid_f<T>(raw) : 1.0f; }
 
 // ----------------------------------------------------------------------------------------------------------------
 // Forward.  S lanes per channel, NPL states per lane: 64 / S channels per wave, a wave per (channel tile, group, row,
@@ -168,12 +170,12 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
             uu[k] = (float)ru[k];
-            dt[k] = step_width((float)rd[k] + bias, a.softplus);
+            dt[k] = step_width<T>((float)rd[k] + bias, a.softplus);
             du[k] = dt[k] * uu[k];
             sz[k] = 1.0f;
             if (MODE == 0 && a.z) {
                 const float zz = (float)rz[k];
-                sz[k] = zz * sigmoid_f(zz);
+                sz[k] = zz * sigmoid_f<T>(zz);
             }
             if (MODE == 1 && k * S + q < left) sum_dt += dt[k];
         }
@@ -556,10 +558,10 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     // tokens behind the row's last and lanes without a channel: width 0 (decay 1), and they add nothing
-                    w[j] = j < count ? step_width(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
+                    w[j] = j < count ? step_width<T>(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
                     x[j] = w[j] * gu[k].at(j);
                     const float zz = gz[k].at(j);
-                    o[j] = gated ? gy[k].at(j) * (zz * sigmoid_f(zz)) : gy[k].at(j);
+                    o[j] = gated ? gy[k].at(j) * (zz * sigmoid_f<T>(zz)) : gy[k].at(j);
                 }
                 if (i < Q) {
                     store<float, 4>(&width[i][slot], w);
@@ -691,10 +693,10 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const float skip = param[1][slot + j], uu = gu[k].at(j), out = gy[k].at(j), zz = gz[k].at(j);
-                            const float sg = sigmoid_f(zz), gg = gated ? out * (zz * sg) : out;
+                            const float sg = sigmoid_f<T>(zz), gg = gated ? out * (zz * sg) : out;
                             ou[j] = in ? fmaf(s1[j], w[j], gg * skip) : 0.0f;
                             // sum of through A = sum of through A2, times ln 2
-                            od[j] = in ? fmaf(s1[j], uu, s2[j] * kLn2) * step_slope(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
+                            od[j] = in ? fmaf(s1[j], uu, s2[j] * kLn2) * step_slope<T>(gd[k].at(j) + param[0][slot + j], softplus) : 0.0f;
                             oz[j] = in ? out * fmaf(skip, uu, sy[j]) * (sg * fmaf(zz, 1.0f - sg, 1.0f)) : 0.0f;
                             dbias[j] += od[j];
                             if (in) dD[j] = fmaf(gg, uu, dD[j]);
@@ -821,7 +823,7 @@ __global__ __launch_bounds__(kStepThreads) void k_scan_step(ScanArgs a) {
     for (; b < a.B; b += step) {
         float h[4], x[4], C[4];
         const float u = (float)ru, z = (float)rz;
-        const float dt = step_width((float)rd + bias, a.softplus);
+        const float dt = step_width<T>((float)rd + bias, a.softplus);
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[j] = mark ? 0.0f : rh.at(j), x[j] = dt * u * rB.at(j), C[j] = rC.at(j);
         ask(b + step);
@@ -835,7 +837,7 @@ __global__ __launch_bounds__(kStepThreads) void k_scan_step(ScanArgs a) {
         put(a.new_state + (b * a.D + d) * a.N + q * 4, count, h);
         if (q == 0) {
             acc = fmaf(skip, u, acc);
-            if (a.z) acc *= z * sigmoid_f(z);
+            if (a.z) acc *= z * sigmoid_f<T>(z);
             ((T*)a.y)[b * a.y_row + d] = (T)acc;
         }
     }

@@ -94,16 +94,20 @@ constexpr float kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// e^x with the product x log2(e) carried to twice the width: e^x = 2^(hi + lo), 2^lo = 1 + lo ln 2.  Without the low
-// part the rounding of the product alone costs |x| 2^-24 of relative error.
+// e^x for activations of type T.  The rounding of the product x log2(e) moves the result by |x| 2^-24 of itself: nothing
+// beside what a 16-bit x was rounded by itself, but for 32-bit ones the product is carried to twice the width,
+// e^x = 2^(hi + lo), 2^lo = 1 + lo ln 2.
+template <class T>
 __device__ __forceinline__ float exp_f(float x) {
     const float hi = x * kLog2e;
+    if constexpr (sizeof(T) == 2) return exp2_hw(hi);
     // (infinite x: the low part is NaN, which the median of three turns into a finite number; e is then 0, infinite or NaN)
     const float lo = __builtin_amdgcn_fmed3f(fmaf(x, kLog2eLow, fmaf(x, kLog2e, -hi)), -1.0f, 1.0f);
     return exp2_hw(hi) * fmaf(lo, kLn2, 1.0f);
 }
 
-__device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f(-x)); }
+template <class T>
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f<T>(-x)); }
 
 // log(1 + e) for 0 <= e <= 1: 2 artanh(s), s = e / (2 + e) <= 1/3, by its series; the first term left out is
 // s^17 / 17 <= 5e-10, below the last place of s.  No cancellation for small e, unlike log(1 + e) itself.
@@ -121,8 +125,9 @@ __device__ __forceinline__ float log1p_unit(float e) {
 }
 // softplus(x) = log(1 + e^x) = max(x, 0) + log(1 + e^-|x|); its derivative is the sigmoid, from the same exponential.
 // Both select with comparisons that are false for NaN, so NaN comes out as NaN.
+template <class T>
 __device__ __forceinline__ float softplus_f(float x) {
-    const float e = exp_f(-__builtin_fabsf(x));
+    const float e = exp_f<T>(-__builtin_fabsf(x));
     return (x < 0.0f ? 0.0f : x) + log1p_unit(e);
 }
 
