@@ -19,12 +19,14 @@ int64_t tiles_of(const auv_scan_args& p, int64_t lanes) { return ceil_div(p.chan
 struct Chunks {
     int64_t length, count;
 };
-// Splits the time axis when the rows alone leave the chip short of waves.  A split pays for itself only when it brings
-// at least three chunks: every element is then gone over twice.  (7 rows x 1,001 tokens x 90 channels, forwards and
-// backwards: 105 us with two waves per SIMD and chunks of 32 tokens at least, 71 us with four and 16.)
-Chunks split(int64_t L, int64_t waves) {
-    constexpr int64_t kEnough = 1024, kTarget = 4096;   // one and four waves per SIMD of the 256 CUs
-    if (waves >= kEnough) return {L, 1};
+// Splits the time axis when the rows alone leave the chip short of waves: fewer than `enough`, which is one wave per SIMD
+// of the 256 CUs forwards and two backwards.  A split pays for itself only when it brings at least three chunks: every
+// element is then gone over twice.  16 states, 128 channels, 512 tokens, bf16: 128 rows backwards 288 us in four chunks,
+// 470 us whole; 512 rows forwards 187 us whole, 362 us in chunks.  (7 rows x 1,001 tokens x 90 channels, forwards and
+// backwards: 105 us with chunks for two waves per SIMD and of 32 tokens at least, 71 us for four and of 16.)
+Chunks split(int64_t L, int64_t waves, int64_t enough) {
+    constexpr int64_t kTarget = 4096;   // four waves per SIMD
+    if (waves >= enough) return {L, 1};
     const int64_t want = ceil_div(kTarget, waves);
     int64_t length = ceil_div(ceil_div(L, want), kSegment) * kSegment;
     const int64_t count = ceil_div(L, length);
@@ -32,7 +34,9 @@ Chunks split(int64_t L, int64_t waves) {
 }
 
 struct Forward {
-    bool narrow;     // four states per lane instead of sixteen: four times the waves for small batches
+    // four states per lane instead of sixteen: four times the waves for small batches.  16 states, 128 channels, 512 tokens,
+    // bf16: 512 rows 187 us narrow, 245 us wide; 768 rows 269 and 326; 1,024 rows (two wide waves per SIMD) 327 us wide.
+    bool narrow;
     int64_t waves;   // without chunks
     Chunks chunks;
 };
@@ -42,7 +46,7 @@ Forward forward_plan(const auv_scan_args& p) {
     const int64_t wide = tiles_of(p, S > 4 ? S / 4 : 1) * p.groups * p.batch;
     f.narrow = S > 1 && wide < 2048;
     f.waves = f.narrow ? tiles_of(p, S) * p.groups * p.batch : wide;
-    f.chunks = split(p.length, f.waves);
+    f.chunks = split(p.length, f.waves, 1024);
     return f;
 }
 
@@ -60,7 +64,7 @@ Backward backward_plan(const auv_scan_args& p) {
     r.blocks = ceil_div(tiles, r.per);
     r.grid_y = r.blocks * p.groups;
     const int64_t groups = ceil_div(p.batch, r.units);
-    r.chunks = split(p.length, groups * r.grid_y * waves);
+    r.chunks = split(p.length, groups * r.grid_y * waves, 2048);
     // each workgroup leaves one record of sums per row it works on side by side: as many as fill the chip, not more
     const int64_t cap = r.grid_y < 1024 ? 1024 / r.grid_y : 1;
     r.grid_x = groups * r.chunks.count < cap ? groups * r.chunks.count : cap;
