@@ -1,6 +1,8 @@
 // auv_residual_norm: checks, launch rules and launches of auv_norm.hpp.
 #include "auv_seq_host.hpp"
 
+#include <cfloat>
+
 #include "auv_norm.hpp"
 
 namespace auv {
@@ -30,7 +32,8 @@ int check(const auv_norm_args& p, int32_t pass) {
         return seq_fail(AUV_ERR_ARG, "%s: the residual stream is f32 or of the block's type", who);
     if (p.channels > AUV_NORM_MAX_CHANNELS)
         return seq_fail(AUV_ERR_ARG, "%s: at most %d channels, got %lld", who, AUV_NORM_MAX_CHANNELS, (long long)p.channels);
-    if (!(p.eps > 0.0)) return seq_fail(AUV_ERR_ARG, "%s: eps must be positive", who);
+    // (as a normal number of 32 bits: a row of zeros rests on it)
+    if (!((float)p.eps >= FLT_MIN)) return seq_fail(AUV_ERR_ARG, "%s: eps must be positive in 32 bits", who);
     if (p.gate_act < AUV_GATE_PLAIN || p.gate_act > AUV_GATE_SIGMOID) return seq_fail(AUV_ERR_ARG, "%s: unknown gate activation", who);
     return AUV_OK;
 }

@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * kJoinRows) void k_scan_join(JoinArgs a) {
         for (int64_t c = c0; c < c1; ++c) {
             const float s = a.chunk_state[at(c)], q = a.chunk_decay[at(c)];
             h = join(q, h, s);
-            p *= q;
+            p = q == 0.0f ? 0.0f : p * q;       // (p may be an infinity or NaN by now)
         }
     }
     hs[row][lane] = h;
@@ -637,8 +637,8 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
                         const float B = bc[i][0][q * 4 + j];
                         x1 = j == 0 ? dh * B : fmaf(dh, B, x1);
                         carry[j] = dh * exp2_hw(w * A2[j]);
-                        if (STARTS && (marks >> i & 1)) carry[j] = 0.0f;
-                        const float through = carry[j] * hist[m][j];
+                        float through = carry[j] * hist[m][j];
+                        if (STARTS && (marks >> i & 1)) carry[j] = through = 0.0f;   // (hist may be anything here)
                         x2 = j == 0 ? through * A2[j] : fmaf(through, A2[j], x2);
                         dA[j] = fmaf(through, w, dA[j]);
                     }

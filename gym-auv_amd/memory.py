@@ -33,6 +33,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
 import weakref
 
 import torch
@@ -46,6 +47,7 @@ TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib
 GATES = {None: _lib.GATE_PLAIN, "silu": _lib.GATE_SILU, "sigmoid": _lib.GATE_SIGMOID}
 MAX_STATES = 64
 WIDTHS = (2, 3, 4)
+_LEAST = torch.finfo(torch.float32).smallest_normal
 
 
 # ----------------------------------------------------------------------------
@@ -129,10 +131,11 @@ def _apart(name, t, other_name, o):
 
 
 def _in_place(name, lo, t, others):
-    """A step's new state, t's worth of memory from address lo on, holds none of the step's inputs (by their addresses)."""
+    """A step's new state, t's worth of memory from address lo on, shares none with the step's inputs, each given as its
+    address and its length up to the last byte."""
     hi = lo + t.numel() * t.element_size()
-    for p in others:
-        if lo <= p < hi:
+    for p, n in others:
+        if p < hi and lo < p + n:
             raise ValueError(f"{name} holds an input of the step")
 
 
@@ -149,32 +152,45 @@ def _no_grad_here(who, tensors):
         raise RuntimeError(f"{who} keeps no gradients: call it under torch.no_grad(), or use the form for whole rollouts")
 
 
-class _EagerGraph:
-    """Lives as long as the graph node of an eager call; names the leaves it accumulates into (which the node keeps alive)."""
-    __slots__ = ("leaves", "__weakref__")
-
-    def __init__(self, leaves):
-        self.leaves = leaves
+_eager_nodes = weakref.WeakSet()     # the graph nodes of eager calls, as long as their graphs live
+_eager_lock = threading.Lock()
 
 
-_eager_graphs = weakref.WeakSet()
+def _leaves_of(nodes):
+    """The leaves whose gradient accumulators lie behind these graph nodes."""
+    leaves, seen, todo = set(), set(), list(nodes)
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)       # an accumulator's
+        if leaf is not None:
+            leaves.add(id(leaf))
+        todo.extend(n for n, _ in node.next_functions)
+    return leaves
 
 
-def _mark_graph(tensors):
+def _check_capture(tensors):
     """Refuse to record a graph whose backward pass would end in gradient accumulators that an eager graph made: torch
-    runs those on the eager graph's stream, and joining that stream to a capture ends the process.  Returns what the
-    call's own node is to keep."""
-    leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
-    if not leaves:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        if any(leaves & g.leaves for g in list(_eager_graphs)):
-            raise RuntimeError("a graph that records gradients is being captured while the outputs of an earlier eager pass "
-                               "over the same parameters are alive: drop those first")
-        return None
-    mark = _EagerGraph(leaves)
-    _eager_graphs.add(mark)
-    return mark
+    runs those on the eager graph's stream, and joining that stream to a capture ends the process."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    with _eager_lock:
+        alive = _leaves_of(_eager_nodes)
+    if not alive:
+        return
+    wanted = [t for t in tensors if t is not None and t.requires_grad]
+    leaves = {id(t) for t in wanted if t.grad_fn is None}
+    if (leaves | _leaves_of(t.grad_fn for t in wanted)) & alive:
+        raise RuntimeError("a graph that records gradients is being captured while the outputs of an earlier eager pass "
+                           "over the same parameters are alive: drop those first")
+
+
+def _note_node(ctx):
+    if not torch.cuda.is_current_stream_capturing():
+        with _eager_lock:
+            _eager_nodes.add(ctx)
 
 
 def _ptr(t):
@@ -192,6 +208,13 @@ def _rows(t):
 def _groups(t):
     s = t.stride()
     return t.data_ptr(), s[0], s[1], s[2]
+
+
+def _new(t, dtype=None):
+    """Memory for a result of t's shape, in t's layout where that leaves the channels adjacent (a sliding window over a
+    signal has two strides of 1, and may come back the other way round)."""
+    r = torch.empty_like(t, dtype=dtype)
+    return r if r.stride(-1) == 1 or t.shape[-1] <= 1 else torch.empty(t.shape, dtype=r.dtype, device=t.device)
 
 
 def _adjacent(t):
@@ -240,7 +263,7 @@ def _conv_head(x, weight, bias, start, lengths, state, silu):
 
 
 def _conv_forward(x, weight, bias, start, lengths, state, silu, return_state):
-    y = torch.empty_like(x)
+    y = _new(x)
     new = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if return_state else None
     if x.numel() == 0:
         if return_state:
@@ -253,10 +276,11 @@ def _conv_forward(x, weight, bias, start, lengths, state, silu, return_state):
 
 class _Conv(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, state, start, lengths, silu, return_state, mark):
+    def forward(ctx, x, weight, bias, state, start, lengths, silu, return_state):
+        _note_node(ctx)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, state, start, lengths)
-        ctx.silu, ctx.mark = silu, mark
+        ctx.silu = silu
         return _conv_forward(x, weight, bias, start, lengths, state, silu, return_state)
 
     @staticmethod
@@ -264,14 +288,14 @@ class _Conv(torch.autograd.Function):
     def backward(ctx, dy, dnew):
         x, weight, bias, state, start, lengths = ctx.saved_tensors
         want_x, want_w, want_b, want_s = ctx.needs_input_grad[:4]
-        rest = (None,) * 5
+        rest = (None,) * 4
         if x.numel() == 0:
             zeros = lambda t, want: torch.zeros_like(t) if want else None   # noqa: E731
             ds = None if not want_s else torch.zeros_like(state) if dnew is None else dnew.clone()
             return (zeros(x, want_x), zeros(weight, want_w), zeros(bias, want_b), ds) + rest
-        dy = torch.zeros_like(x) if dy is None else _adjacent(dy)
+        dy = _new(x).zero_() if dy is None else _adjacent(dy)
         dnew = None if dnew is None else dnew.contiguous()
-        dx = torch.empty_like(x)
+        dx = _new(x)
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(bias) if want_b else None
         ds = torch.empty_like(state) if want_s else None
@@ -306,7 +330,8 @@ def causal_conv(x, weight, bias=None, *, start=None, lengths=None, state=None, s
     _dense("state", state, (B, W - 1, D), dev, x.dtype)
     silu, tensors = 1 if silu else 0, (x, weight, bias, state)
     if _wants_grad(tensors):
-        y, new = _Conv.apply(*tensors, start, lengths, silu, bool(return_state), _mark_graph(tensors))
+        _check_capture(tensors)
+        y, new = _Conv.apply(*tensors, start, lengths, silu, bool(return_state))
     else:
         y, new = _conv_forward(x, weight, bias, start, lengths, state, silu, return_state)
     return (y, new) if return_state else y
@@ -326,7 +351,9 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, (B, W - 1, D), dev, x.dtype)
         _apart("new_state", new_state, "state", state)
-    _in_place("the new state", to, state, (x.data_ptr(), weight.data_ptr(), _ptr(bias), marks[0]))
+    size, last = x.element_size(), max(B - 1, 0)
+    _in_place("the new state", to, state, ((x.data_ptr(), (last * strides[0] + D) * size), (weight.data_ptr(), 4 * D * W),
+                                           (_ptr(bias), 4 * D if bias is not None else 0), (marks[0], last * marks[1] + 1 if start is not None else 0)))
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
     if B and D:
         block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
@@ -340,7 +367,7 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
 # ----------------------------------------------------------------------------
 def _scan_forward(u, A, state, head, return_state, keep):
     """`head`: the argument block up to state."""
-    y = torch.empty_like(u)
+    y = _new(u)
     new = torch.empty((u.shape[0],) + tuple(A.shape), dtype=torch.float32, device=u.device) if return_state else None
     if u.numel() == 0:
         if return_state:
@@ -360,11 +387,12 @@ def _scan_forward(u, A, state, head, return_state, keep):
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, head, return_state, mark):
+    def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, head, return_state):
+        _note_node(ctx)
         ctx.set_materialize_grads(False)
         y, new, segments = _scan_forward(u, A, state, head, return_state, True)
         ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, segments)
-        ctx.softplus, ctx.mark = head[7], mark
+        ctx.softplus = head[7]
         return y, new
 
     @staticmethod
@@ -372,17 +400,17 @@ class _Scan(torch.autograd.Function):
     def backward(ctx, dy, dnew):
         u, delta, A, Bm, Cm, D, z, delta_bias, state, start, lengths, segments = ctx.saved_tensors
         want = ctx.needs_input_grad
-        rest = (None,) * 5
+        rest = (None,) * 4
         if u.numel() == 0:
             out = [torch.zeros_like(t) if w else None
                    for t, w in zip((u, delta, A, Bm, Cm, D, z, delta_bias, state), want)]
             if want[8] and dnew is not None:
                 out[8] = dnew.clone()
             return (*out, *rest)
-        dy = torch.zeros_like(u) if dy is None else _adjacent(dy)
+        dy = _new(u).zero_() if dy is None else _adjacent(dy)
         dnew = None if dnew is None else dnew.contiguous()
-        du, ddelta, dB, dC = torch.empty_like(u), torch.empty_like(delta), torch.empty_like(Bm), torch.empty_like(Cm)
-        dz = None if z is None else torch.empty_like(z)
+        du, ddelta, dB, dC = _new(u), _new(delta), _new(Bm), _new(Cm)
+        dz = None if z is None else _new(z)
         dA = torch.empty_like(A) if want[2] else None
         dD = torch.empty_like(D) if want[5] else None
         dbias = torch.empty_like(delta_bias) if want[7] else None
@@ -445,7 +473,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_
     head = _scan_head(u, shape, strides, dev, delta, A, B, C, D, z, delta_bias, start, lengths, state, delta_softplus, False)
     tensors = (u, delta, A, B, C, D, z, delta_bias, state)
     if _wants_grad(tensors):
-        y, new = _Scan.apply(*tensors, start, lengths, head, bool(return_state), _mark_graph(tensors))
+        _check_capture(tensors)
+        y, new = _Scan.apply(*tensors, start, lengths, head, bool(return_state))
     else:
         y, new, _ = _scan_forward(u, A, state, head, return_state, False)
     return (y, new) if return_state else y
@@ -462,7 +491,12 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, state.shape, dev)
         _apart("new_state", new_state, "state", state)
-    _in_place("the new state", to, state, (head[8], head[11], head[14], head[17], head[21], *head[25:29]))
+    # (address and row stride of u, delta, z, B, C and start lie at these places of the block)
+    (B_, D_), N, G, size, last = shape, head[5], head[6], u.element_size(), max(shape[0] - 1, 0)
+    _in_place("the new state", to, state, (
+        *((head[i], (last * head[i + 1] + D_) * size) for i in (8, 11, 14) if head[i]),
+        *((head[i], (last * head[i + 1] + (G - 1) * head[i + 3] + N) * size) for i in (17, 21)),
+        (head[25], 4 * D_ * N), *((head[i], 4 * D_) for i in (26, 27) if head[i]), *((head[28], last * head[29] + 1),) * bool(head[28])))
     y = torch.empty(shape, dtype=u.dtype, device=u.device)
     if shape[0] and shape[1]:
         block = _pack_scan(*head, to, y.data_ptr(), shape[1], 0, *(0,) * 26)
@@ -487,8 +521,8 @@ def _norm_head(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
 
 
 def _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
-    out = torch.empty_like(x) if y is not None else None
-    h = torch.empty_like(x if y is None else y, dtype=dtype) if pre_weight is not None else None
+    out = _new(x) if y is not None else None
+    h = _new(x if y is None else y, dtype) if pre_weight is not None else None
     if x.numel():
         head = _norm_head(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
         _call("auv_residual_norm", _pack_norm(*head, *_rows(out), *_rows(h), *(0,) * 18), _lib.SEQ_FORWARD, head[0], scratch=False)
@@ -497,10 +531,11 @@ def _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
 
 class _Norm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, post_weight, pre_weight, gate, scale, act, eps, dtype, mark):
+    def forward(ctx, x, y, post_weight, pre_weight, gate, scale, act, eps, dtype):
+        _note_node(ctx)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, post_weight, pre_weight, gate, scale)
-        ctx.how, ctx.mark = (act, eps, dtype), mark
+        ctx.how = (act, eps, dtype)
         return _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
 
     @staticmethod
@@ -508,14 +543,14 @@ class _Norm(torch.autograd.Function):
     def backward(ctx, d_out, d_h):
         x, y, post_weight, pre_weight, gate, scale = ctx.saved_tensors
         want = ctx.needs_input_grad
-        rest = (None,) * 4
+        rest = (None,) * 3
         if d_out is None and d_h is None or x.numel() == 0:
             return tuple(torch.zeros_like(t) if w else None
                          for t, w in zip((x, y, post_weight, pre_weight, gate, scale), want)) + rest
         d_out, d_h = _adjacent(d_out), _adjacent(d_h)
-        dx = torch.empty_like(x)
-        dy = None if y is None else torch.empty_like(y)
-        dgate = None if gate is None else torch.empty_like(gate)
+        dx = _new(x)
+        dy = None if y is None else _new(y)
+        dgate = None if gate is None else _new(gate)
         dpost = torch.empty_like(post_weight) if want[2] else None
         dpre = torch.empty_like(pre_weight) if want[3] else None
         dscale = torch.empty_like(scale) if want[5] else None
@@ -530,8 +565,8 @@ def _norm(x, dev, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype)
     D = x.shape[-1]
     if D < 1 or D > _lib.NORM_MAX_CHANNELS:
         raise ValueError(f"1 to {_lib.NORM_MAX_CHANNELS} channels, got {D}")
-    if not eps > 0.0:
-        raise ValueError("eps must be positive")
+    if not eps >= _LEAST:
+        raise ValueError("eps must be positive in 32 bits")
     if gate_act not in GATES:
         raise ValueError(f"gate_act must be one of {tuple(GATES)}, got {gate_act!r}")
     _dense("post_weight", post_weight, (D,), dev)
@@ -542,7 +577,8 @@ def _norm(x, dev, y, post_weight, pre_weight, gate, scale, gate_act, eps, dtype)
     if len(shape) != 3:
         x, y, gate = _as_rows(x), _as_rows(y), _as_rows(gate)
     if _wants_grad(tensors):
-        out, h = _Norm.apply(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype, _mark_graph(tensors))
+        _check_capture(tensors)
+        out, h = _Norm.apply(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
     else:
         out, h = _norm_forward(x, y, post_weight, pre_weight, gate, scale, act, eps, dtype)
     if len(shape) != 3:

@@ -103,6 +103,13 @@ def test_c_entry_points_refuse(lib, fn, args, what, match):
     assert rc < 0 and match in lib.auv_seq_last_error().decode()
 
 
+def test_an_eps_that_vanishes_in_32_bits_is_refused(lib):
+    """A row of zeros would divide by it."""
+    assert lib.auv_residual_norm(C.byref(norm_args(eps=1e-60)), _lib.SEQ_FORWARD, None) < 0
+    assert b"eps" in lib.auv_seq_last_error()
+    assert lib.auv_residual_norm_workspace(C.byref(norm_args(eps=1e-60)), _lib.SEQ_BACKWARD) < 0
+
+
 def test_c_entry_points_refuse_null_blocks(lib):
     for fn in ("auv_causal_conv", "auv_selective_scan", "auv_residual_norm"):
         assert getattr(lib, fn)(None, 0, None) == -1

@@ -330,6 +330,73 @@ def test_an_episode_does_not_see_what_came_before():
         assert torch.equal(yc[:, cut:], memory.causal_conv(x[:, cut:], w, b))
 
 
+@pytest.mark.parametrize("B,L,cut", [(2, 900, 700), (2, 900, 16), (3, 700, 333), (1, 1500, 1300)])
+def test_what_a_start_parts_in_a_row_of_many_chunks(B, L, cut):
+    """Rows cut into chunks, one episode before `cut` and one from there on: neither sees NaN or infinities in any of the
+    other's tokens, widths and gradients included."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(17, "float32", "time")
+    D, N = 20, 16
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, True, True)
+    gy = m.rows(B, L, D)
+    start = torch.zeros(B, L, dtype=torch.uint8, device="cuda")
+    start[:, cut] = 1
+    rows, names = ("u", "delta", "B", "C", "z"), ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
+    K = 10 * (L + N + 12)
+    for part in (slice(cut, None), slice(0, cut)):
+        first = part.start == 0
+        spoilt = {k: v if v is None else v.detach().clone() for k, v in t.items()}
+        hole = slice(cut, None) if first else slice(0, cut)
+        g = gy.clone()
+        for i, v in enumerate([*(spoilt[k] for k in rows), g]):
+            v[:, hole] = float("nan") if i % 2 == 0 else float("inf")
+        spoilt["delta"][:, hole] = float("nan")
+        if not first:
+            spoilt["state"].fill_(float("inf"))
+        given = [spoilt[k].requires_grad_(True) for k in names]
+        y = memory.selective_scan(*given, start=start, state=spoilt["state"])
+        grads = torch.autograd.grad(y, [spoilt[k] for k in rows], g)
+        alone = {k: v if v is None or k not in rows else v[:, part] for k, v in t.items()}
+        if not first:
+            alone["state"] = None
+        want = scan_oracle(alone, None, None, gy[:, part])
+        check("y", y[:, part], want["y"], K)
+        for k, d in zip(rows, grads):
+            check("d_" + k, d[:, part], want[k], 2 * K + D)
+
+
+def test_windows_that_overlap():
+    """Sliding windows over a signal: channels adjacent, and the next token one element on."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(18, "float32")
+    D, N, L = 30, 4, 11
+    signal = m.par(2, L + D - 1)
+    x = signal.unfold(1, D, 1)
+    assert x.shape == (2, L, D) and x.stride()[1:] == (1, 1)
+    w, wn, A = m.par(D, 4), m.par(D), -m.par(D, N).abs()
+    bc = m.rows(2, L, 1, N)
+    gy = m.rows(2, L, D)
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        outs = [memory.causal_conv(x, w), memory.selective_scan(x, x, A, bc, bc, z=x)]
+        return outs + [torch.autograd.grad(o, x, gy)[0] for o in outs]
+
+    for a, b in zip(run(x), run(x.contiguous())):
+        assert torch.equal(a, b)
+    x, y = x.detach().requires_grad_(True), x.detach().requires_grad_(True)      # (two leaves over the same memory)
+    outs = memory.residual_norm(x, y, wn, wn)
+    grads = torch.autograd.grad(outs, [x, y], [gy, gy])
+    flat = lambda t: host(t).reshape(-1, D)                                       # noqa: E731
+    want = O.norm(flat(x), flat(y), host(wn), host(wn), dx_out=flat(gy), dh=flat(gy))
+    for name, t in (("x_out", outs[0]), ("h", outs[1]), ("x", grads[0]), ("y", grads[1])):
+        check(name, t, tuple(v.reshape(t.shape) for v in want[name]), 4 * (D + 24) + 2 * L)
+
+
 # ----------------------------------------------------------------------------
 # norms
 # ----------------------------------------------------------------------------
@@ -492,6 +559,30 @@ def test_a_step_does_not_read_what_it_writes():
         memory.causal_conv_step(s[:, 1], s, torch.zeros(8, 4, device="cuda"))
 
 
+def test_a_step_does_not_read_what_it_writes_from_an_earlier_start():
+    """Inputs that begin before the state's memory and reach into it, and ones that end where it begins."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    buf = torch.zeros(2048, device="cuda")
+    h, A, bc = buf[256:512].view(2, 8, 16), torch.zeros(8, 16, device="cuda"), torch.zeros(2, 1, 16, device="cuda")
+    x = torch.zeros(2, 8, device="cuda")
+    for bad in (buf[200:].as_strided((2, 8), (56, 1)), buf[255:263].expand(2, 8), buf[252:268].view(2, 8)):
+        with pytest.raises(ValueError, match="holds an input"):
+            memory.selective_scan_step(bad, x, h, A, bc, bc)
+        with pytest.raises(ValueError, match="holds an input"):
+            memory.causal_conv_step(bad, buf[256:304].view(2, 3, 8), torch.zeros(8, 4, device="cuda"))
+    with pytest.raises(ValueError, match="holds an input"):
+        memory.selective_scan_step(x, x, h, buf[200:328].view(8, 16), bc, bc)
+    with pytest.raises(ValueError, match="holds an input"):
+        memory.selective_scan_step(x, x, h, A, bc, buf[226:258].view(2, 1, 16))
+    with pytest.raises(ValueError, match="holds an input"):
+        memory.causal_conv_step(x, buf[256:304].view(2, 3, 8), buf[225:257].view(8, 4))
+    ahead = buf[240:256].view(2, 8)
+    memory.selective_scan_step(ahead, ahead, h, A, bc, bc)
+    memory.causal_conv_step(ahead, buf[256:304].view(2, 3, 8), torch.zeros(8, 4, device="cuda"))
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 elements: the last rows, computed within the whole and by themselves.  (Rows of the same shape go
     through the same kernels with the same bits.)"""
@@ -651,6 +742,28 @@ def test_capturing_gradients_beside_a_live_eager_graph_is_refused():
     g.replay()
     torch.cuda.synchronize()
     assert float(gw.abs().sum()) == 0.0
+
+
+def test_capturing_beside_a_live_eager_graph_of_the_leaves_behind_the_arguments():
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    u, bc = torch.zeros(2, 5, 8, device="cuda"), torch.zeros(2, 5, 1, 4, device="cuda")
+    log_A, w = torch.zeros(8, 4, device="cuda", requires_grad=True), torch.ones(8, 4, device="cuda", requires_grad=True)
+    alive = memory.selective_scan(u, u, -torch.exp(log_A), bc, bc)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="drop those first"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            memory.selective_scan(u, u, -torch.exp(log_A), bc, bc)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="drop those first"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            memory.causal_conv(u, log_A)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):       # other leaves: recorded
+        memory.causal_conv(u, w)
+    torch.cuda.synchronize()
+    del alive
 
 
 def test_step_captured_with_its_state_in_place():
