@@ -16,11 +16,11 @@ int64_t lanes_of(int64_t channels) {
 }
 int64_t rows_of(int64_t lanes) { return lanes < 256 ? 256 / lanes : 1; }
 
-// Workgroups of a backward pass: each leaves one record of column sums, so a workgroup takes many rows.  768 of 256
-// threads are three per CU, all that the registers hold (262,144 rows of 250 channels: forward and backward 590 us; with
-// 2,048, the last of which start when the first end, 630 us).
+// Workgroups of a backward pass: each leaves one record of column sums, so a workgroup takes many rows.  512 of 256
+// threads are two per CU, all that the registers hold (262,144 rows of 250 channels, forward and backward: 487 us; with
+// 768, the last of which start when the first end, 504 us).
 int64_t back_blocks(int64_t rows, int64_t channels) {
-    const int64_t lanes = lanes_of(channels), want = ceil_div(rows, rows_of(lanes)), cap = lanes == 1024 ? 256 : 768;
+    const int64_t lanes = lanes_of(channels), want = ceil_div(rows, rows_of(lanes)), cap = lanes == 1024 ? 256 : 512;
     return want < cap ? want : cap;
 }
 

@@ -116,6 +116,30 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
     put((T*)a.h_out + b * a.h_row + l * a.h_token + d, count, r);
 }
 
+// A lane's elements of a row: all of them where its vector is whole (rows of more than 32 channels), or the first `count`.
+template <int TPR, class T, int V>
+__device__ __forceinline__ void fetch_row(Raw<T, V>& out, const T* p, int count) {
+    fetch(out, p, TPR > 4 ? V : count);
+}
+template <int TPR, class T, int V>
+__device__ __forceinline__ void put_row(T* p, int count, const float (&in)[V]) {
+    if constexpr (TPR > 4) {
+        if (count) store<T, V>(p, in);
+    } else {
+        put(p, count, in);
+    }
+}
+
+// The kernel's arguments, read where they are used: some fifty addresses and strides held in scalar registers through the
+// row loop would push each other out to vector lanes.
+__device__ __forceinline__ NormArgs norm_args() {
+    const __attribute__((address_space(4))) NormArgs* p = (const __attribute__((address_space(4))) NormArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    NormArgs r;
+    __builtin_memcpy(&r, (const NormArgs*)p, sizeof(NormArgs));
+    return r;
+}
+
 // Gradients.  x' is formed again from x, y and gate in 32 bits (its stored form may be rounded), then
 //
 //   t = gh pre_weight            dr = gx + r2 t - x' r2^3 mean(t x')            dx = dr
@@ -125,75 +149,94 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
 // A lane owns the same columns of every row its workgroup works on, so the three sums over rows stay in registers and
 // leave as one record per workgroup.  The next row's elements are asked for before the sums of this one.
 template <class TR, class T, int TPR>
-__global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
+__global__ __launch_bounds__(norm_threads<TPR>(), 2) void k_norm_backward(NormArgs a) {
     constexpr int TH = norm_threads<TPR>(), ROWS = TH / TPR, V = kNormLane;
     // by sum and, turn about, by row: whichever sums a call leaves out, a barrier lies between two uses of a buffer
     __shared__ float buf_y[2][TH / 64][1], buf_x[2][TH / 64][2], buf_n[2][TH / 64][1];
     int turn = 0;
     __shared__ float fold[ROWS > 1 ? TH * V : 1];
-    const int d = threadIdx.x % TPR * V, slot = threadIdx.x / TPR;
+    const int slot = threadIdx.x / TPR, D = (int)a.D, d_lane = threadIdx.x % TPR * V;
+    // A lane takes whole vectors: where V does not divide the channels, the last lane takes the last V, `shared` of which
+    // its neighbour has as well.  Both form and write the same values; the sums take them from the neighbour.  Lanes
+    // without channels read what the last one reads, and rows behind the last what that one holds, so that no load is
+    // masked; they write nothing and count for nothing.
+    const bool whole = TPR > 4;
+    const int mine = d_lane >= D ? 0 : whole || D >= V ? V : D;
+    const int d = (whole || mine == V) && d_lane > D - V ? D - V : d_lane, shared = d_lane - d < V ? d_lane - d : V;
     const int64_t rows = a.B * a.L;
-    const int mine = clamp_count(a.D - d, V);
-    const float inv = 1.0f / (float)a.D;
+    const float inv = 1.0f / (float)D;
+    const bool with_y = a.y != nullptr, gated = a.gate != nullptr, post = a.post_weight != nullptr, with_h = a.gh != nullptr;
+    const int kind = a.act;
     float w1[V], w2[V], sc[V], d1[V], d2[V], ds[V];
+    auto column = [&](const float* from, float absent, float (&to)[V]) {
+        Raw<float, V> t;
+        if (from) fetch_row<TPR>(t, from + d, mine);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        w1[v] = v < mine && a.post_weight ? a.post_weight[d + v] : 1.0f;
-        w2[v] = v < mine && a.pre_weight ? a.pre_weight[d + v] : 0.0f;
-        sc[v] = v < mine && a.scale ? a.scale[d + v] : 1.0f;
-        d1[v] = d2[v] = ds[v] = 0.0f;
-    }
+        for (int v = 0; v < V; ++v) to[v] = from ? t.at(v) : absent;
+    };
+    column(a.post_weight, 1.0f, w1);
+    column(a.pre_weight, 0.0f, w2);
+    column(a.scale, 1.0f, sc);
+#pragma unroll
+    for (int v = 0; v < V; ++v) d1[v] = d2[v] = ds[v] = 0.0f;
+    // the row's place is moved on, not divided out of its number, from one row to the next
+    const int64_t first = (int64_t)blockIdx.x * ROWS, step = (int64_t)gridDim.x * ROWS, step_b = step / a.L, step_l = step - step_b * a.L;
+    int64_t b, l, next_b = (first + slot) / a.L, next_l = first + slot - next_b * a.L;
     Raw<TR, V> fx = {}, fgx = {};
     Raw<T, V> fy = {}, fg = {}, fgh = {};
     auto ask = [&](int64_t row) {
+        const NormArgs r = norm_args();
         const int count = row < rows ? mine : 0;
-        const int64_t b = row < rows ? row / a.L : 0, l = row < rows ? row - b * a.L : 0;
-        fetch(fx, (const TR*)a.x + b * a.x_row + l * a.x_token + d, count);
-        if (a.y) fetch(fy, (const T*)a.y + b * a.y_row + l * a.y_token + d, count);
-        if (a.gate) fetch(fg, (const T*)a.gate + b * a.gate_row + l * a.gate_token + d, count);
-        if (a.gx) fetch(fgx, (const TR*)a.gx + b * a.gx_row + l * a.gx_token + d, count);
-        if (a.gh) fetch(fgh, (const T*)a.gh + b * a.gh_row + l * a.gh_token + d, count);
+        if (whole && row >= rows) next_b = r.B - 1, next_l = r.L - 1;
+        fetch_row<TPR>(fx, (const TR*)r.x + next_b * r.x_row + next_l * r.x_token + d, count);
+        if (r.y) fetch_row<TPR>(fy, (const T*)r.y + next_b * r.y_row + next_l * r.y_token + d, count);
+        if (r.gate) fetch_row<TPR>(fg, (const T*)r.gate + next_b * r.gate_row + next_l * r.gate_token + d, count);
+        if (r.gx) fetch_row<TPR>(fgx, (const TR*)r.gx + next_b * r.gx_row + next_l * r.gx_token + d, count);
+        if (r.gh) fetch_row<TPR>(fgh, (const T*)r.gh + next_b * r.gh_row + next_l * r.gh_token + d, count);
     };
-    const int64_t first = (int64_t)blockIdx.x * ROWS, step = (int64_t)gridDim.x * ROWS;
     ask(first + slot);
     for (int64_t row0 = first; row0 < rows; row0 += step, turn ^= 1) {
         const int64_t row = row0 + slot;
         const int count = row < rows ? mine : 0;
-        const int64_t b = row < rows ? row / a.L : 0, l = row < rows ? row - b * a.L : 0;
+        b = next_b, l = next_l;
         float r[V], y[V], dr[V], t[V], act[V], slope[V];
         float s1[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            r[v] = fx.at(v), y[v] = fy.at(v), dr[v] = fgx.at(v), t[v] = fgh.at(v);
+            r[v] = fx.at(v), y[v] = fy.at(v), dr[v] = count ? fgx.at(v) : 0.0f, t[v] = count ? fgh.at(v) : 0.0f;
             act[v] = slope[v] = 1.0f;
-            s1[0] = fmaf(y[v], y[v], s1[0]);
+            s1[0] = fmaf(v >= shared ? y[v] : 0.0f, y[v], s1[0]);
         }
-        if (a.gate) {
+        if (gated && kind == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) act[v] = fg.at(v);
+        } else if (gated) {
+            const bool silu = kind == 1;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float g = fg.at(v);
-                act[v] = g;
-                if (a.act != 0) {
-                    const float s = sigmoid_f<T>(g);
-                    act[v] = a.act == 1 ? g * s : s;
-                    slope[v] = a.act == 1 ? s * fmaf(g, 1.0f - s, 1.0f) : s * (1.0f - s);
-                }
+                const float g = fg.at(v), s = sigmoid_f<T>(g);
+                act[v] = s * (silu ? g : 1.0f);
+                slope[v] = fmaf(act[v], 1.0f - s, silu ? s : 0.0f);    // SiLU: s (1 + g (1 - s)); sigmoid: s (1 - s)
             }
         }
+        next_b += step_b, next_l += step_l;
+        if (next_l >= a.L) next_l -= a.L, ++next_b;
         ask(row + step);
         float r1 = 1.0f;
-        if (a.post_weight) {
+        if (post) {
             row_sum<TPR, 1>(s1, buf_y[turn]);
             r1 = __builtin_amdgcn_rsqf(fmaf(s1[0], inv, a.eps));
         }
-        float s2[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            r[v] = fmaf(sc[v] * act[v], y[v] * (r1 * w1[v]), r[v]);
-            s2[0] = fmaf(r[v], r[v], s2[0]);
-            s2[1] = fmaf(t[v] * w2[v], r[v], s2[1]);
-        }
-        if (a.gh) {
+        for (int v = 0; v < V; ++v) r[v] = fmaf(sc[v] * act[v], y[v] * (r1 * w1[v]), r[v]);
+        if (with_h) {
+            float s2[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float once = v >= shared ? r[v] : 0.0f;
+                s2[0] = fmaf(once, r[v], s2[0]);
+                s2[1] = fmaf(t[v] * w2[v], once, s2[1]);
+            }
             row_sum<TPR, 2>(s2, buf_x[turn]);
             const float r2 = __builtin_amdgcn_rsqf(fmaf(s2[0], inv, a.eps));
             const float back = s2[1] * inv * r2 * r2 * r2;
@@ -203,8 +246,9 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
                 dr[v] += fmaf(r2 * w2[v], t[v], -r[v] * back);
             }
         }
-        if (a.dx) put((TR*)a.dx + b * a.dx_row + l * a.dx_token + d, count, dr);
-        if (!a.dy) continue;
+        const NormArgs to = norm_args();
+        if (to.dx) put_row<TPR>((TR*)to.dx + b * to.dx_row + l * to.dx_token + d, count, dr);
+        if (!with_y) continue;
         s1[0] = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -213,35 +257,39 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
             slope[v] *= dr[v] * sc[v] * n;                          // dgate
             t[v] = dr[v] * sc[v] * act[v];                          // dn
             d1[v] = fmaf(t[v], y[v] * r1, d1[v]);
-            s1[0] = fmaf(t[v] * w1[v], y[v], s1[0]);
+            s1[0] = fmaf(t[v] * w1[v], v >= shared ? y[v] : 0.0f, s1[0]);
         }
-        if (a.dgate) put((T*)a.dgate + b * a.dgate_row + l * a.dgate_token + d, count, slope);
+        if (to.dgate) put_row<TPR>((T*)to.dgate + b * to.dgate_row + l * to.dgate_token + d, count, slope);
         float through = 0.0f;
-        if (a.post_weight) {
+        if (post) {
             row_sum<TPR, 1>(s1, buf_n[turn]);
             through = s1[0] * inv * r1 * r1 * r1;
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) t[v] = fmaf(r1 * w1[v], t[v], -y[v] * through);
-        put((T*)a.dy + b * a.dy_row + l * a.dy_token + d, count, t);
+        put_row<TPR>((T*)to.dy + b * to.dy_row + l * to.dy_token + d, count, t);
     }
     if (!a.partial) return;
     auto leave = [&](const float (&v)[V], int which) {
-        if (ROWS > 1) {
+        float* const to = a.partial + (int64_t)blockIdx.x * a.D * 3 + which;
+        if constexpr (ROWS > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < V; ++i) fold[threadIdx.x * V + i] = v[i];
             __syncthreads();
-        }
-        if (slot == 0) {
+#pragma unroll 1
+            for (int e = threadIdx.x; e < TPR * V; e += TH) {
+                // element e % V of lane e / V, whose vector may have moved up from where it belongs
+                const int at = e / V * V, from = D >= V && at > D - V ? D - V : at, column = from + e % V;
+                if (at >= D || column < at || column >= D) continue;
+                float sum = 0.0f;
+                for (int w = 0; w < ROWS; ++w) sum += fold[w * TPR * V + e];
+                to[(int64_t)column * 3] = sum;
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (i < mine) {
-                    float s = ROWS > 1 ? 0.0f : v[i];
-                    if (ROWS > 1)
-                        for (int w = 0; w < ROWS; ++w) s += fold[w * TPR * V + d + i];
-                    a.partial[((int64_t)blockIdx.x * a.D + d + i) * 3 + which] = s;
-                }
+                if (i >= shared && i < mine) to[(int64_t)(d + i) * 3] = v[i];
         }
     };
     leave(d1, 0);
