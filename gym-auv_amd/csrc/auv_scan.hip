@@ -66,6 +66,8 @@ Backward backward_plan(const auv_scan_args& p) {
     const int64_t groups = ceil_div(p.batch, r.units);
     r.chunks = split(p.length, groups * r.grid_y * waves, 2048);
     // each workgroup leaves one record of sums per row it works on side by side: as many as fill the chip, not more
+    // (4,096 rows x 64 tokens x 128 channels, 16 states, forwards and backwards: 890 us; with half of them 896, with four
+    // times as many 917)
     const int64_t cap = r.grid_y < 1024 ? 1024 / r.grid_y : 1;
     r.grid_x = groups * r.chunks.count < cap ? groups * r.chunks.count : cap;
     const int64_t NP = 4 * S;
@@ -180,7 +182,8 @@ template <class T, int S>
 int run_step(ScanArgs a, hipStream_t stream) {
     const int64_t lanes = a.D * S < kStepThreads ? a.D * S : kStepThreads, tiles = ceil_div(a.D * S, lanes);
     a.lanes = (int32_t)lanes;
-    // eight workgroups per CU, each with as many rows as it takes
+    // eight workgroups per CU, each with as many rows as it takes (65,536 rows of 64 channels, 16 states: 126 us; two per CU
+    // 153 us; a workgroup for every row 181 us)
     const int64_t want = ceil_div(a.B, kStepThreads / lanes), most = ceil_div(2048, tiles);
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)tiles), block(kStepThreads);
     hipLaunchKernelGGL((k_scan_step<T, S>), grid, block, 0, stream, a);

@@ -8,8 +8,11 @@
 // handed on are those after the row's last token.  Everything between the loads and the one rounding of each output is
 // in 32 bits.
 //
-// Two bounds lie close together: 4 elements of traffic per (token, channel), and per state one exponential, two
-// multiplications and two fused multiply-adds on the vector unit.
+// Two bounds lie close together: 4 elements of traffic per (token, channel), and per state one exponential (two issue
+// slots), two multiplications and two fused multiply-adds on the vector unit.  4,096 rows x 128 tokens x 128 channels, bf16,
+// 16 states: the traffic (638 MB) asks for 124 us, 96 slots for the states and some 45 for widths, gates, sums and their
+// loads and stores for 290 us.  It takes 296 to 328 us with the vector unit busy 90 % of the time: bound by arithmetic.
+// The product x B as a rank-1 matrix instruction (4 x 4 x 1, in 32 bits) took 444 us, C h by them as well 506 us.
 #pragma once
 
 #include <type_traits>
@@ -70,17 +73,18 @@ __device__ __forceinline__ float step_slope(float raw, int softplus) { return so
 
 // ----------------------------------------------------------------------------------------------------------------
 // Forward.  S lanes per channel, NPL states per lane: 64 / S channels per wave, a wave per (channel tile, group, row,
-// chunk of time).  With S > 1 the lanes of a channel share the element-wise work of its tokens.  B and C of the next tokens go through LDS once per wave as floats, zero-padded to NP states, which
-// takes care of odd counts and strides; every lane of a channel reads them from there at the same address.
+// chunk of time).  With S > 1 the lanes of a channel share the element-wise work of its tokens.  B and C of the next tokens
+// go through LDS once per wave as floats, zero-padded to NP states, which takes care of odd counts and strides; every lane
+// of a channel reads them from there at the same address.
 //
 // MODE 0 computes outputs (from `state`, or from the chunk's entry state when the row is split into chunks).
 // MODE 1 starts each chunk from zero and leaves only its end state and its decay, exp(A sum dt) (0 behind a start).
 // ----------------------------------------------------------------------------------------------------------------
 template <int S>
 constexpr int lane_bits() { return S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0; }
-template <int S>
 // Tokens at a time: at least one for every lane of a channel.  Four where a lane has whole channels: eight take 233
 // registers (two waves per SIMD, 398 us for 4,096 x 128 x 128 in bf16 with 16 states), four 165 (three, 356 us).
+template <int S>
 constexpr int scan_tile() { return S > 8 ? S : S == 1 ? 4 : 8; }
 
 template <class T, int NPL, int S, int MODE>
@@ -317,7 +321,10 @@ __global__ __launch_bounds__(64 * kJoinRows) void k_scan_join(JoinArgs a) {
 // The element-wise parts (widths, gates and their derivatives; the stores of du, ddelta, dz) belong to the workgroup: a
 // thread takes four adjacent channels of a token, so that loads and stores are 8 or 16 bytes wide and a token's channels
 // go in one piece.  Two-byte accesses by the lanes of the sweeps, 32 bytes of a token at a time, took longer than the
-// arithmetic.
+// arithmetic.  4,096 rows x 64 tokens x 128 channels, bf16, 16 states: 700 us (1,878 us in the first form, with lanes that
+// loaded for themselves and sums through shuffles) at 2,360 vector instructions per 16 tokens of 16 channels, the vector
+// unit busy 82 % of the time: bound by arithmetic.  The element-wise parts take 15 % of it, the tokens gone over twice in
+// half segments 7 %, the fetching 5 %, the sums of dB and dC 4 %.
 template <int S>
 constexpr int scan_back_waves() { return S <= 4 ? 8 : 4; }
 // tokens whose states a lane holds at a time: half a segment, so that two waves more fit on a SIMD (with S = 16 the sums
@@ -785,7 +792,8 @@ __global__ __launch_bounds__(256) void k_scan_sum_bc(ScanArgs a, int NP, int blo
 // One token per row: the states once in, once out, 8 N bytes per channel against some 50 bytes of everything else.  A
 // lane holds 4 states, S lanes a channel, so that a wave reads 1 KiB of adjacent states per load; it keeps its channel's
 // parameters for all the rows it takes and asks for the next row's states while it works on one.  state and new_state may
-// be the same memory: a lane writes only what it alone has read.
+// be the same memory: a lane writes only what it alone has read.  65,536 rows x 64 channels x 16 states: 117 to 126 us (575
+// MB, 4.6 to 4.9 TB/s); 146 us with parameters fetched for every row and nothing asked for ahead.
 // ----------------------------------------------------------------------------------------------------------------
 constexpr int kStepThreads = 256;
 template <class T, int S>

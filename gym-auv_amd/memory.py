@@ -351,9 +351,9 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, (B, W - 1, D), dev, x.dtype)
         _apart("new_state", new_state, "state", state)
-    size, last = x.element_size(), max(B - 1, 0)
-    _in_place("the new state", to, state, ((x.data_ptr(), (last * strides[0] + D) * size), (weight.data_ptr(), 4 * D * W),
-                                           (_ptr(bias), 4 * D if bias is not None else 0), (marks[0], last * marks[1] + 1 if start is not None else 0)))
+    last, pb = B - 1 if B else 0, _ptr(bias)
+    _in_place("the new state", to, state, ((x.data_ptr(), (last * strides[0] + D) * x.element_size()), (weight.data_ptr(), 4 * D * W),
+                                           (pb, 4 * D), (marks[0], last * marks[1] + 1)))
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
     if B and D:
         block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
@@ -491,12 +491,13 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
     if new_state is not None and new_state is not state:
         to = _dense("new_state", new_state, state.shape, dev)
         _apart("new_state", new_state, "state", state)
-    # (address and row stride of u, delta, z, B, C and start lie at these places of the block)
-    (B_, D_), N, G, size, last = shape, head[5], head[6], u.element_size(), max(shape[0] - 1, 0)
+    # (addresses and row strides as they lie in the block; an absent tensor's address is 0, below any state)
+    (_, _, rows, _, chans, N, G, _, pu, su, _, pd, sd, _, pz, sz, _, pB, sB, _, gB, pC, sC, _, gC, pA, pD, pb, ps, ss) = head[:30]
+    last, size, more = rows - 1 if rows else 0, u.element_size(), G - 1
     _in_place("the new state", to, state, (
-        *((head[i], (last * head[i + 1] + D_) * size) for i in (8, 11, 14) if head[i]),
-        *((head[i], (last * head[i + 1] + (G - 1) * head[i + 3] + N) * size) for i in (17, 21)),
-        (head[25], 4 * D_ * N), *((head[i], 4 * D_) for i in (26, 27) if head[i]), *((head[28], last * head[29] + 1),) * bool(head[28])))
+        (pu, (last * su + chans) * size), (pd, (last * sd + chans) * size), (pz, (last * sz + chans) * size),
+        (pB, (last * sB + more * gB + N) * size), (pC, (last * sC + more * gC + N) * size),
+        (pA, 4 * chans * N), (pD, 4 * chans), (pb, 4 * chans), (ps, last * ss + 1)))
     y = torch.empty(shape, dtype=u.dtype, device=u.device)
     if shape[0] and shape[1]:
         block = _pack_scan(*head, to, y.data_ptr(), shape[1], 0, *(0,) * 26)
