@@ -336,7 +336,7 @@ __device__ __forceinline__ void put_with_halo(float* row, int Lo, int lo, float 
 typedef float cnn_float2 __attribute__((ext_vector_type(2)));
 
 // The two conv positions under a pooled cell share every weight: they are the
-// two halves of one packed fused multiply-add.  Tap k needs (x[k], x[k+1]):
+// two halves of a pair (two fused multiply-adds each).  Tap k needs (x[k], x[k+1]):
 // even taps take the pairs (x0,x1) (x2,x3) ..., odd taps the pairs (x1,x2) ...
 template <int CIN, int COUT, int L, bool LAST>
 __device__ __forceinline__ void deep_conv(const float* in, float* out, const float* w, const float* b, int lane) {

@@ -10,8 +10,8 @@ thread_local char g_seq_error[512];
 
 // Tokens per thread.  A run re-reads the W - 1 tokens before it, so long runs read less; short ones give a small batch
 // more threads.  Runs of 32 wherever that leaves two waves per SIMD of the 256 CUs (131,072 threads), down to 8.  4,096
-// rows x 128 tokens x 128 channels, bf16, forwards and backwards: 172 us in runs of 32, 229 us in runs of 8; 7 rows of up
-// to 1,001 tokens x 90 channels forwards, with the launch: 25 us and 16 us.
+// rows x 128 tokens x 128 channels, bf16, forwards and backwards: 172 us in runs of 32, 229 us in runs of 8; 5 rows of up
+// to 4,001 tokens x 90 channels forwards, with the launch: 25 us and 16 us.
 int conv_run(int64_t B, int64_t L, int64_t vectors) {
     int run = 32;
     while (run > 8 && B * ceil_div(L, run) * vectors < 131072) run /= 2;
