@@ -354,10 +354,10 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
     last, pb = B - 1 if B else 0, _ptr(bias)
     _in_place("the new state", to, state, ((x.data_ptr(), (last * strides[0] + D) * x.element_size()), (weight.data_ptr(), 4 * D * W),
                                            (pb, 4 * D), (marks[0], last * marks[1] + 1)))
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    y = _new(x)
     if B and D:
         block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
-                           _ptr(bias), *marks, 0, s, to, y.data_ptr(), D, 0, *(0,) * 10)
+                           pb, *marks, 0, s, to, y.data_ptr(), y.stride(0), 0, *(0,) * 10)
         _call("auv_causal_conv", block, _lib.SEQ_STEP, dev, scratch=False)
     return y
 
@@ -498,9 +498,9 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
         (pu, (last * su + chans) * size), (pd, (last * sd + chans) * size), (pz, (last * sz + chans) * size),
         (pB, (last * sB + more * gB + N) * size), (pC, (last * sC + more * gC + N) * size),
         (pA, 4 * chans * N), (pD, 4 * chans), (pb, 4 * chans), (ps, last * ss + 1)))
-    y = torch.empty(shape, dtype=u.dtype, device=u.device)
+    y = _new(u)
     if shape[0] and shape[1]:
-        block = _pack_scan(*head, to, y.data_ptr(), shape[1], 0, *(0,) * 26)
+        block = _pack_scan(*head, to, y.data_ptr(), y.stride(0), 0, *(0,) * 26)
         _call("auv_selective_scan", block, _lib.SEQ_STEP, dev, scratch=False)
     return y
 
