@@ -261,8 +261,9 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
 
 // Joins the chunks of a row: chunk_state[c] becomes the state the chunk starts from (forwards from `state`) or, going
 // backwards, the gradient that reaches the chunk's last state from behind (from the gradient of the states handed on,
-// which lands in dstate at the front).  A workgroup takes 64 numbers and splits the chunks over 16 rows of threads.
-constexpr int kJoinRows = 16;
+// which lands in dstate at the front).  A workgroup takes LANES numbers and splits the chunks over 1,024 / LANES rows of
+// threads.  Bound by the latency of its loads: few numbers want many rows.
+constexpr int kJoinThreads = 1024;
 struct JoinArgs {
     float *chunk_state, *chunk_decay;
     const float* first;     // [B,D,N] or null
@@ -270,12 +271,14 @@ struct JoinArgs {
     int64_t chunks, count;  // count = B D NP
     int32_t N, NP, reverse;
 };
-__global__ __launch_bounds__(64 * kJoinRows) void k_scan_join(JoinArgs a) {
-    __shared__ float hs[kJoinRows][64], ps[kJoinRows][64];
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+template <int LANES>
+__global__ __launch_bounds__(kJoinThreads) void k_scan_join(JoinArgs a) {
+    constexpr int ROWS = kJoinThreads / LANES;
+    __shared__ float hs[ROWS][LANES], ps[ROWS][LANES];
+    const int lane = threadIdx.x % LANES, row = threadIdx.x / LANES;
+    const int64_t i = (int64_t)blockIdx.x * LANES + lane;
     const bool live = i < a.count;
-    const int64_t per = (a.chunks + kJoinRows - 1) / kJoinRows;
+    const int64_t per = (a.chunks + ROWS - 1) / ROWS;
     const int64_t c0 = row * per < a.chunks ? row * per : a.chunks, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
     auto at = [&](int64_t c) { return (a.reverse ? a.chunks - 1 - c : c) * a.count + i; };
     // a decay of exactly 0 cuts: whatever came before (also an infinity) has no part in what follows
@@ -297,13 +300,19 @@ __global__ __launch_bounds__(64 * kJoinRows) void k_scan_join(JoinArgs a) {
     const int s = (int)(i - bd * a.NP);
     float x = a.first && s < a.N ? a.first[bd * a.N + s] : 0.0f;
     for (int r = 0; r < row; ++r) x = join(ps[r][lane], x, hs[r][lane]);
-#pragma unroll 4
-    for (int64_t c = c0; c < c1; ++c) {
-        const float e = a.chunk_state[at(c)], q = a.chunk_decay[at(c)];
-        a.chunk_state[at(c)] = x;
-        x = join(q, x, e);
+    for (int64_t c = c0; c < c1; c += 4) {      // four at a time: no load waits behind the stores before it
+        float e[4], q[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (c + k < c1) e[k] = a.chunk_state[at(c + k)], q[k] = a.chunk_decay[at(c + k)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (c + k < c1) {
+                a.chunk_state[at(c + k)] = x;
+                x = join(q[k], x, e[k]);
+            }
     }
-    if (a.last && s < a.N && row == kJoinRows - 1) a.last[bd * a.N + s] = x;
+    if (a.last && s < a.N && row == ROWS - 1) a.last[bd * a.N + s] = x;
 }
 
 // ----------------------------------------------------------------------------------------------------------------

@@ -367,6 +367,29 @@ def test_what_a_start_parts_in_a_row_of_many_chunks(B, L, cut):
             check("d_" + k, d[:, part], want[k], 2 * K + D)
 
 
+@pytest.mark.parametrize("B,L,D,N,ragged,share", [(2, 4200, 12, 16, None, 0.002), (1, 4128, 30, 7, None, 0.0), (3, 4100, 5, 20, "ragged", 0.001)])
+def test_scan_of_a_few_long_rows_against_the_oracle(B, L, D, N, ragged, share):
+    """Hundreds of chunks a row, joined forwards and backwards, from a state and to the gradient of one."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(19, "float32", "time")
+    t, start, n = scan_case(m, B, L, D, N, 1, share, ragged, True, True)
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    args = [t[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")]
+    y, new = memory.selective_scan(*args, start=start, lengths=n, state=t["state"], return_state=True)
+    names = list(t)
+    grads = torch.autograd.grad([y, new], [t[k] for k in names], [gy, gs])
+    want = scan_oracle(t, start, n, gy, gs)
+    # (a decay carried over C chunks takes C products where the oracle takes L: no more roundings than the bound counts)
+    K = 10 * (L + N + 12)
+    check("y", y, want["y"], K)
+    check("new_state", new, want["new_state"], K)
+    for name, g in zip(names, grads):
+        more = B * L if name in ("A", "D", "delta_bias") else D if name in ("B", "C") else 0
+        check("d_" + name, g, want[name], 2 * K + more)
+
+
 def test_windows_that_overlap():
     """Sliding windows over a signal: channels adjacent, and the next token one element on."""
     torch = torch_()
