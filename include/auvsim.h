@@ -596,7 +596,7 @@ int auv_selective_scan(const auv_scan_args* args, int32_t pass, void* stream);
 typedef struct auv_norm_args {
     int64_t device, dtype, residual_dtype, batch, length, channels;
     int64_t gate_act;
-    double eps;
+    double eps;                   /* at least the smallest normal number of 32 bits */
     const void* x;
     int64_t x_row, x_token;
     const void* y;
