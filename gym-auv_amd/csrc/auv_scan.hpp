@@ -43,7 +43,7 @@ struct ScanArgs {
     int64_t y_row, y_token;
     float* segments;         // [B, ceil(L/16), D, NP]: the states before every 16th token
     int64_t chunk, chunks;   // tokens per chunk (a multiple of 16), chunks per row
-    float *chunk_state, *chunk_decay;   // [chunks, B, D, NP]
+    float *chunk_state, *chunk_decay;   // [chunks, B, D, NP]; decays as chunk_log gives them
     // backward
     const void* dy;
     int64_t dy_row, dy_token;
@@ -78,8 +78,15 @@ __device__ __forceinline__ float step_slope(float raw, int softplus) { return so
 // of a channel reads them from there at the same address.
 //
 // MODE 0 computes outputs (from `state`, or from the chunk's entry state when the row is split into chunks).
-// MODE 1 starts each chunk from zero and leaves only its end state and its decay, exp(A sum dt) (0 behind a start).
+// MODE 1 starts each chunk from zero and leaves only its end state and its decay, exp(A sum dt), as its logarithm.
 // ----------------------------------------------------------------------------------------------------------------
+// A chunk's decay is handed on as its logarithm (to base 2): the decay itself leaves the 32 bits' range long before what it
+// is a factor of does, 16 tokens that each take e^-6, or give it, suffice.  Kept finite, so that logarithms can be added
+// up; negative infinity stands for a start within the chunk and for nothing else.  (A step width that is no number makes
+// the chunk's own end state one that is none, whatever stands here.)
+constexpr float kCut = -__builtin_inff();
+__device__ __forceinline__ float chunk_log(bool cut, float log) { return cut ? kCut : __builtin_amdgcn_fmed3f(log, -1e30f, 1e30f); }
+
 template <int S>
 constexpr int lane_bits() { return S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0; }
 // Tokens at a time: at least one for every lane of a channel.  Four where a lane has whole channels: eight take 233
@@ -245,7 +252,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
 #pragma unroll
             for (int j = 0; j < NPL; ++j) {
                 a.chunk_state[o + j] = h[j];
-                a.chunk_decay[o + j] = cut ? 0.0f : exp2_hw(sum_dt * A2[j]);
+                a.chunk_decay[o + j] = chunk_log(cut, sum_dt * A2[j]);
             }
         }
         return;
@@ -281,15 +288,20 @@ __global__ __launch_bounds__(kJoinThreads) void k_scan_join(JoinArgs a) {
     const int64_t per = (a.chunks + ROWS - 1) / ROWS;
     const int64_t c0 = row * per < a.chunks ? row * per : a.chunks, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
     auto at = [&](int64_t c) { return (a.reverse ? a.chunks - 1 - c : c) * a.count + i; };
-    // a decay of exactly 0 cuts: whatever came before (also an infinity) has no part in what follows
-    auto join = [](float p, float x, float s) { return p == 0.0f ? s : fmaf(p, x, s); };
-    float h = 0.0f, p = 1.0f;
+    // s + 2^p x.  Behind a start whatever came before (also an infinity or NaN) has no part in what follows.  Everywhere else
+    // it has one: 2^p is multiplied in by halves within [2^-126, 2^127], so that an infinity or NaN stays one however small the
+    // decay, a 0 stays 0 however large, and what is cut off at either end is off by less than 2^-124, or beyond 2^128 too.
+    auto join = [](float p, float x, float s) {
+        const float r = exp2_hw(__builtin_amdgcn_fmed3f(0.5f * p, -126.0f, 127.0f));
+        return p == kCut ? s : fmaf(x * r, r, s);
+    };
+    float h = 0.0f, p = 0.0f;
     if (live) {
 #pragma unroll 4
         for (int64_t c = c0; c < c1; ++c) {
             const float s = a.chunk_state[at(c)], q = a.chunk_decay[at(c)];
             h = join(q, h, s);
-            p = q == 0.0f ? 0.0f : p * q;       // (p may be an infinity or NaN by now)
+            p += q;
         }
     }
     hs[row][lane] = h;
@@ -753,7 +765,7 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     r.chunk_state[o + j] = carry[j];
-                    r.chunk_decay[o + j] = cut ? 0.0f : exp2_hw(sum_dt * A2[j]);
+                    r.chunk_decay[o + j] = chunk_log(cut, sum_dt * A2[j]);
                 }
             }
         } else if (r.dstate && r.chunks == 1 && live && on) {

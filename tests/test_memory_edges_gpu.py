@@ -1,0 +1,125 @@
+"""The sequence operators at the edges of what they take: values that are not finite, states that vanish or
+grow, sizes beyond one launch, and calls that other torch machinery makes."""
+import numpy as np
+import pytest
+
+from oracle import seq_oracle as O
+from tests.test_memory_gpu import TYPES, Maker, check, host, hostb, lengths_of, scan_case, torch_
+
+pytestmark = pytest.mark.gpu
+
+SCAN_ARGS = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
+
+
+def finite_alike(name, got, want, K):
+    """`got` is finite exactly where the definition is a number that got's type holds, and within its bound there.  (A state
+    that grows by 2^134 hands back gradients beyond 2^128, which 64 bits hold and 32 do not.)"""
+    import torch
+
+    value, magnitude = want
+    fin = np.abs(value) <= torch.finfo(got.dtype).max           # (false for NaN)
+    have = torch.isfinite(got.detach()).cpu().numpy()
+    same = np.array_equal(have, fin)
+    assert same, (name, "finite:", int(have.sum()), "should be:", int(fin.sum()), "of", fin.size, "first at",
+                                       tuple(int(i) for i in np.argwhere(have != fin)[0]))
+    keep = torch.from_numpy(fin).to(got.device)
+    check(name, torch.where(keep, got.detach(), torch.zeros_like(got)),
+          (np.where(fin, value, 0.0), np.where(fin, np.nan_to_num(magnitude, nan=0.0, posinf=0.0), 0.0)), K)
+
+
+def raw_scan(t, start, n, gy, gs, softplus):
+    """The oracle on the values as they are, with nothing cleaned."""
+    v = {k: host(x) for k, x in t.items()}
+    with np.errstate(all="ignore"):
+        return O.scan(*(v[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")), softplus, hostb(start),
+                      None if n is None else n.cpu().numpy(), v["state"], host(gy), host(gs))
+
+
+def run_scan(t, start, n, gy, gs, softplus):
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    t = {k: None if v is None else v.detach().requires_grad_(True) for k, v in t.items()}
+    y, new = memory.selective_scan(*(t[k] for k in SCAN_ARGS), delta_softplus=softplus, start=start, lengths=n, state=t["state"],
+                                   return_state=True)
+    names = [k for k, v in t.items() if v is not None]
+    return dict(y=y, new_state=new, **dict(zip(names, torch.autograd.grad([y, new], [t[k] for k in names], [gy, gs]))))
+
+
+# ----------------------------------------------------------------------------
+# rows cut into chunks: what one chunk hands to the next
+# ----------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("where", ["u", "state", "d_y", "d_state"])
+def test_what_is_not_finite_goes_on_to_the_next_start(where, bad):
+    """A decays every state by e^-8 a token, by e^-128 (0 in 32 bits) over 16 tokens: a value that is not finite still
+    stays until an episode starts, forwards, and back to the episode's first token, backwards."""
+    torch = torch_()
+    m = Maker(31, "float32", "time")
+    B, L, D, N = 2, 700, 20, 16
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, True, True)
+    t["A"] = torch.full_like(t["A"], -16.0)
+    t["delta"], t["delta_bias"] = torch.full_like(t["delta"], 0.5), None
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    start = torch.zeros(B, L, dtype=torch.bool, device="cuda")
+    start[0, 400], start[1, 200] = True, True
+    put = {"u": t["u"], "state": t["state"], "d_y": gy, "d_state": gs}[where]
+    if where == "u":
+        put[0, 3, 5] = float(bad)
+    elif where == "d_y":
+        put[0, 650, 5] = float(bad)
+    else:
+        put[0, 5, 2] = float(bad)
+    got, want = run_scan(t, start, None, gy, gs, False), raw_scan(t, start, None, gy, gs, False)
+    K = 10 * (L + N + 12)
+    assert not np.isfinite(want["y" if where in ("u", "state") else "u"][0][0]).all()
+    for name in ("y", "new_state"):
+        finite_alike(name, got[name], want[name], K)
+    for name in ("u", "delta", "z", "B", "C", "A", "D", "state"):
+        finite_alike("d_" + name, got[name], want[name], 2 * K + (B * L if name in ("A", "D") else D))
+
+
+@pytest.mark.parametrize("B,L", [(2, 700), (1, 4200)])
+def test_states_that_grow(B, L):
+    """e^8 a token, beyond 32 bits over 16 tokens: states that are 0 stay 0, backwards too, until something feeds them."""
+    torch = torch_()
+    m = Maker(32, "float32", "time")
+    D, N = 20, 16
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, False, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    t["A"], t["delta"], t["delta_bias"] = torch.full_like(t["A"], 16.0), torch.full_like(t["delta"], 0.5), None
+    t["u"][:, :-3] = 0
+    gy, gs = m.rows(B, L, D), torch.zeros(B, D, N, device="cuda")
+    gy[:, 3:] = 0
+    got, want = run_scan(t, None, None, gy, gs, False), raw_scan(t, None, None, gy, gs, False)
+    # (three tokens that grow: each exponent 8 log2(e) = 11.5 rounded twice, a relative 2 x 8 of a step each)
+    K = 10 * (L + N + 12) + 3 * 16
+    for name in got:
+        assert np.isfinite(want[name][0]).all()
+        finite_alike(name, got[name], want[name], 2 * K + B * L)
+
+
+def test_a_state_that_grows_by_more_than_32_bits_hold():
+    """By 2^134 within a chunk, from 1e-30 to 2e10: the product of the decays alone is no number."""
+    torch = torch_()
+    m = Maker(33, "float32", "time")
+    B, L, D, N = 1, 100, 20, 16
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, True, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    t["A"], t["delta"], t["delta_bias"] = torch.full_like(t["A"], 11.6), torch.zeros_like(t["delta"]), None
+    t["delta"][:, :16] = 0.5
+    t["u"][:] = 0
+    t["state"] = torch.full_like(t["state"], 1e-30)
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    gy[:, 16:] *= 1e-20
+    gs *= 1e-20
+    got, want = run_scan(t, None, None, gy, gs, False), raw_scan(t, None, None, gy, gs, False)
+    # sixteen tokens whose exponents, 8.4 each, are rounded twice; over a chunk one exponent of 134, rounded 18 times
+    K = 10 * (L + N + 12) + 16 * 2 * 8 + 18 * 134
+    # (one term of dA is d_state times the state before the row: nothing where 32 bits do not hold d_state)
+    held = np.abs(want["state"][0]) <= np.finfo(np.float32).max
+    assert held.any() and not held.all()
+    want["A"] = tuple(np.where(held[0], v, np.nan) for v in want["A"])
+    for name in ("y", "new_state", "state", "A", "C"):
+        finite_alike(name, got[name], want[name], 2 * K + B * L)
