@@ -141,7 +141,7 @@ int run_forward(ScanArgs a, const Forward& f, hipStream_t stream) {
     return launched("k_scan_forward");
 }
 
-template <class T, int S>
+template <class T, int S, bool TAIL>
 int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStream_t stream) {
     static_assert(scan_back_lds<S>(scan_back_waves<S>()) <= 160 * 1024, "the tile's elements and sums must fit the CU's LDS");
     const size_t lds = scan_back_lds<S>((int)r.units);
@@ -149,7 +149,7 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
     static std::atomic<uint64_t> allowed{0};   // devices on which these kernels may take that much LDS
     const uint64_t bit = (uint64_t)1 << (p.device & 63);
     if (lds > 64 * 1024 && (p.device > 63 || !(allowed.load() & bit))) {
-        for (const void* k : {reinterpret_cast<const void*>(&k_scan_backward<T, S, 0>), reinterpret_cast<const void*>(&k_scan_backward<T, S, 1>)}) {
+        for (const void* k : {reinterpret_cast<const void*>(&k_scan_backward<T, S, 0, TAIL>), reinterpret_cast<const void*>(&k_scan_backward<T, S, 1, true>)}) {
             const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                      (int)scan_back_lds<S>(scan_back_waves<S>()));
             if (e != hipSuccess) return seq_fail(AUV_ERR_DEVICE, "k_scan_backward: %zu B of LDS refused: %s", lds, hipGetErrorString(e));
@@ -159,11 +159,11 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
     const dim3 grid((unsigned)r.grid_x, (unsigned)r.grid_y), block(threads);
     if (r.chunks.count > 1) {
         const dim3 all((unsigned)(ceil_div(a.B, r.units) * r.chunks.count), (unsigned)r.grid_y);
-        hipLaunchKernelGGL((k_scan_backward<T, S, 1>), all, block, lds, stream, a);
+        hipLaunchKernelGGL((k_scan_backward<T, S, 1, true>), all, block, lds, stream, a);
         if (const int rc = launched("k_scan_backward")) return rc;
         if (const int rc = join(a, 4 * S, true, stream)) return rc;
     }
-    hipLaunchKernelGGL((k_scan_backward<T, S, 0>), grid, block, lds, stream, a);
+    hipLaunchKernelGGL((k_scan_backward<T, S, 0, TAIL>), grid, block, lds, stream, a);
     if (const int rc = launched("k_scan_backward")) return rc;
     if (a.bc_partial) {
         const int64_t n = ceil_div(a.B * a.L * a.G * 2 * 4 * S, 256);
@@ -179,6 +179,12 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
     s.dst[0] = p.d_A, s.dst[1] = p.d_D, s.dst[2] = p.d_delta_bias;
     hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)ceil_div(s.count, kSumOutputs)), dim3(kSumOutputs * kSumLanes), 0, stream, s);
     return launched("k_seq_sum");
+}
+
+template <class T, int S>
+int by_tail(const ScanArgs& a, const auv_scan_args& p, const Backward& r, hipStream_t stream) {
+    // (4,096 rows x 64 tokens x 128 channels, 16 states: 822 us without the masks for rows that end within a tile, 870 with)
+    return p.lengths || p.length % kSegment ? run_backward<T, S, true>(a, p, r, stream) : run_backward<T, S, false>(a, p, r, stream);
 }
 
 template <class T, int S>
@@ -234,11 +240,11 @@ int by_states(const auv_scan_args& p, int32_t pass, ScanArgs a, hipStream_t stre
     a.partial = (float*)(w + r.chunk_bytes);
     a.bc_partial = r.bc_bytes ? (float*)(w + r.chunk_bytes + r.record_bytes) : nullptr;
     switch (S) {
-        case 1: return run_backward<T, 1>(a, p, r, stream);
-        case 2: return run_backward<T, 2>(a, p, r, stream);
-        case 4: return run_backward<T, 4>(a, p, r, stream);
-        case 8: return run_backward<T, 8>(a, p, r, stream);
-        default: return run_backward<T, 16>(a, p, r, stream);
+        case 1: return by_tail<T, 1>(a, p, r, stream);
+        case 2: return by_tail<T, 2>(a, p, r, stream);
+        case 4: return by_tail<T, 4>(a, p, r, stream);
+        case 8: return by_tail<T, 8>(a, p, r, stream);
+        default: return by_tail<T, 16>(a, p, r, stream);
     }
 }
 

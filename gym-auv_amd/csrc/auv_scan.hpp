@@ -423,13 +423,19 @@ __device__ __forceinline__ int thread_anew() {
 __device__ __forceinline__ int64_t times(int i, int64_t stride) { return (int64_t)((uint64_t)(unsigned)i * (uint64_t)stride); }
 
 // MODE 0: gradients.  MODE 1: from zero at the end of each chunk, only the carry at its front and its decay.
-template <class T, int S, int MODE>
+// TAIL: rows may end within a tile.  The tokens behind have a width of 0, which hands states and carry on as they are; but
+// where these are infinite, 0 times them is not 0, and dA, dB and dC leave such tokens out.
+template <class T, int S, int MODE, bool TAIL>
 __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 : 2) void k_scan_backward(ScanArgs a) {
     constexpr int NP = 4 * S, CW = 64 / S, W = scan_back_waves<S>(), Q = kSegment, HQ = scan_back_hold<S>(), KT = HQ / S, SB = lane_bits<S>();
     constexpr int TH = W * 64, CH = W * CW;
     constexpr int QUADS = CH / 4, STEP = TH / QUADS, IT = Q > STEP ? Q / STEP : 1;   // a thread's tokens: first, first + STEP, ...
     constexpr int BE = Q * 2 * NP / 64;                                             // its share of B and C at the most
     // dB and dC of GT tokens are summed over the wave's channels together: as many values as lanes to sum over
+    // A second form of the sweeps, without the selects for starts and row ends, pays where the registers of both fit: forwards
+    // and backwards, 128 channels x 64 tokens, 8 states 650 us with it and 661 without, 32 states 991 and 1,013, 64 states 1,294
+    // and 1,342; but 16 states (128 registers) 849 and 822, 4 states (256) 596 and 481.
+    constexpr bool kPlainToo = S == 2 || S > 4;
     constexpr int GT = CW >= 8 ? CW / 8 : 1, GV = GT * 8, GR = GV / CW > 1 ? GV / CW : 1;
     static_assert(S <= HQ && GT <= HQ && CW >= 4, "the sums over lanes are formed for whole groups of tokens");
     extern __shared__ __align__(16) float lds[];
@@ -615,9 +621,10 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
                 }
                 continue;
             }
-            // HQ tokens from `first` on, forwards and backwards.  STARTS: some token of the tile opens an episode.
-            auto sweep = [&](auto starts, int first) {
-                constexpr bool STARTS = decltype(starts)::value;
+            // HQ tokens from `first` on, forwards and backwards.  PLAIN: no token of the tile opens an episode or lies behind
+            // the row's last.
+            auto sweep = [&](auto plain, int first) {
+                constexpr bool PLAIN = decltype(plain)::value;
                 float hist[HQ + 1][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) hist[0][j] = h0[j];
@@ -626,7 +633,7 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float before = hist[0][j];
-                        if (STARTS && (marks >> i & 1)) before = 0.0f;
+                        if (!PLAIN && (marks >> i & 1)) before = 0.0f;
                         hist[0][j] = fmaf(exp2_hw(w * A2[j]), before, x * bc[i][0][q * 4 + j]);
                     }
                 }
@@ -640,7 +647,7 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             float before = hist[m][j];
-                            if (STARTS && (marks >> i & 1)) before = 0.0f;
+                            if (!PLAIN && (marks >> i & 1)) before = 0.0f;
                             hist[m + 1][j] = fmaf(exp2_hw(w * A2[j]), before, x * bc[i][0][q * 4 + j]);
                             const float C = bc[i][1][q * 4 + j];
                             part[o] = j == 0 ? hist[m + 1][j] * C : fmaf(hist[m + 1][j], C, part[o]);
@@ -666,7 +673,8 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
                         x1 = j == 0 ? dh * B : fmaf(dh, B, x1);
                         carry[j] = dh * exp2_hw(w * A2[j]);
                         float through = carry[j] * hist[m][j];
-                        if (STARTS && (marks >> i & 1)) carry[j] = through = 0.0f;   // (hist may be anything here)
+                        if (!PLAIN && (marks >> i & 1)) carry[j] = through = 0.0f;   // (hist may be anything here)
+                        if (!PLAIN && TAIL && i >= here) through = 0.0f;
                         x2 = j == 0 ? through * A2[j] : fmaf(through, A2[j], x2);
                         dA[j] = fmaf(through, w, dA[j]);
                     }
@@ -695,8 +703,12 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
             } else {
 #pragma unroll 1
                 for (int first = Q - HQ; first >= 0; first -= HQ) {
-                    if (marks == 0) sweep(std::false_type{}, first);
-                    else sweep(std::true_type{}, first);
+                    if (TAIL && HQ < Q && here <= first) {
+                        for (int e = lane; e < HQ * 2 * NP; e += 64) red[(wave * Q + first) * 2 * NP + e] = 0.0f;
+                        continue;
+                    }
+                    if (kPlainToo && marks == 0 && (!TAIL || here == Q)) sweep(std::true_type{}, first);
+                    else sweep(std::false_type{}, first);
                 }
             }
             __syncthreads();
@@ -749,6 +761,7 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
                     const int64_t br = row0 + un;
                     float sum = 0.0f;
                     for (int w = 0; w < per; ++w) sum += red[((un * per + w) * Q + i) * 2 * NP + which * NP + s];
+                    if (TAIL && t0 + i >= len[un]) sum = 0.0f;
                     if (r.bc_partial)
                         (r.bc_partial + (((int64_t)tb * r.B + br) * r.L + t0) * r.G * 2 * NP)[times(i, r.G * 2 * NP) + (g * 2 + which) * NP + s] = sum;
                     else if (which == 0)

@@ -123,3 +123,45 @@ def test_a_state_that_grows_by_more_than_32_bits_hold():
     want["A"] = tuple(np.where(held[0], v, np.nan) for v in want["A"])
     for name in ("y", "new_state", "state", "A", "C"):
         finite_alike(name, got[name], want[name], 2 * K + B * L)
+
+
+# ----------------------------------------------------------------------------
+# behind a row's last token
+# ----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [3, 7, 16, 20, 64])
+@pytest.mark.parametrize("bad", ["state", "d_state"])
+def test_padding_takes_no_gradient_of_states_that_are_not_finite(bad, N, dtype):
+    torch = torch_()
+    m = Maker(34, dtype, "time")
+    B, L, D = 3, 37, 24
+    t, _, _ = scan_case(m, B, L, D, N, 2, None, None, True, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    n = torch.tensor([L, 5, 18], dtype=torch.int32, device="cuda")
+    {"state": t["state"], "d_state": gs}[bad][:, ::5, 1] = float("inf")
+    got = run_scan(t, None, n, gy, gs, True)
+    for b, k in enumerate(n.tolist()):
+        for name in ("y", "u", "delta", "z", "B", "C"):
+            assert not got[name][b, k:].any(), (name, b)        # (NaN is true)
+
+
+@pytest.mark.parametrize("L,ragged", [(20, False), (33, False), (40, True), (32, False)])
+def test_a_state_that_overflows_with_the_rows_last_token(L, ragged):
+    """The gradients of what came before are finite, A's among them: nothing behind the row's end adds to them."""
+    torch = torch_()
+    m = Maker(35, "float32", "time")
+    B, D, N = 2, 20, 16
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, True, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    n = torch.tensor([23, L], dtype=torch.int32, device="cuda") if ragged else None
+    last = 22 if ragged else L - 1
+    t["delta"][0, last, 5], t["delta_bias"][5] = 3.0, 0.0
+    t["u"][0, last, 5], t["B"][0, last, 0, 2] = 3e38, 100.0
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    got, want = run_scan(t, None, n, gy, gs, True), raw_scan(t, None, n, gy, gs, True)
+    assert np.isfinite(want["A"][0]).all() and np.abs(want["A"][0]).max() < 1e30
+    K = 10 * (L + N + 12)
+    # (the ones that are not a product with dt u of that token, 9e38)
+    for name in ("A", "u", "delta", "D", "delta_bias", "state"):
+        finite_alike(name, got[name], want[name], 2 * K + B * L)
