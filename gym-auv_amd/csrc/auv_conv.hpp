@@ -273,10 +273,15 @@ __global__ __launch_bounds__(kConvThreads, 2) void k_conv_backward(ConvArgs a) {
                                 g *= s * fmaf(pre, 1.0f - s, 1.0f);
                             }
                             gs[i][v] = t < c.real ? g : 0.0f;
-                            const float gc = t < own ? g : 0.0f;
-                            db[v] += gc;
+                        }
+                        // (those behind `own` are left out: 0 times an x that is infinite would be no 0)
+                        if (t < own) {
 #pragma unroll
-                            for (int k = 0; k < W; ++k) dw[v * W + k] = fmaf(gc, xs[(i + 4 - (W - 1) + k) % 4][v], dw[v * W + k]);
+                            for (int v = 0; v < V; ++v) {
+                                db[v] += gs[i][v];
+#pragma unroll
+                                for (int k = 0; k < W; ++k) dw[v * W + k] = fmaf(gs[i][v], xs[(i + 4 - (W - 1) + k) % 4][v], dw[v * W + k]);
+                            }
                         }
                         // dx of token s = t - (W-1), whose g lies in place (i + 5 - W) % 4; token s + k's start is bit W-1-k
                         const int s = t - (W - 1);

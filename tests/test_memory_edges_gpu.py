@@ -165,3 +165,34 @@ def test_a_state_that_overflows_with_the_rows_last_token(L, ragged):
     # (the ones that are not a product with dt u of that token, 9e38)
     for name in ("A", "u", "delta", "D", "delta_bias", "state"):
         finite_alike(name, got[name], want[name], 2 * K + B * L)
+
+
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_last_token_that_is_not_finite_meets_its_own_taps_only(W, dtype):
+    """Without the SiLU the weight gradient is a sum of d_y x: the last token of a row meets the last tap only."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(36, dtype, "time")
+    B, L, D = 3, 21, 24
+    x = m.rows(B, L, D)
+    n = torch.tensor([L, 9, 16], dtype=torch.int32, device="cuda")
+    for b, k in enumerate(n.tolist()):
+        x[b, k - 1, 3 + b] = float("inf")
+    x.requires_grad_(True)
+    w, b = m.par(D, W).requires_grad_(True), m.par(D).requires_grad_(True)
+    gy = m.rows(B, L, D)
+    y = memory.causal_conv(x, w, b, lengths=n, silu=False)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], gy)
+    with np.errstate(all="ignore"):
+        want = O.conv(host(x), host(w), host(b), None, n.cpu().numpy(), None, False, host(gy))
+    assert np.isfinite(want["weight"][0][:, :-1]).all() and not np.isfinite(want["weight"][0][:, -1]).all()
+    # (the oracle's magnitudes of gradients hold those of the pre-activations, which without the SiLU the gradients do not
+    # depend on: they are taken from the row with zeros in place of its infinities)
+    clean = O.conv(np.where(np.isinf(host(x)), 0.0, host(x)), host(w), host(b), None, n.cpu().numpy(), None, False, host(gy))
+    for name in ("x", "weight", "bias"):
+        want[name] = (want[name][0], clean[name][1])
+    K = W + 2 + 8
+    for name, g in (("y", y), ("x", dx), ("weight", dw), ("bias", db)):
+        finite_alike(name, g, want[name], 2 * K + W + B * L)
