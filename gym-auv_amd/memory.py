@@ -139,6 +139,11 @@ def _in_place(name, lo, t, others):
             raise ValueError(f"{name} holds an input of the step")
 
 
+def _written(t):
+    """A kernel has written t: a graph that keeps t for its backward pass has to know, as after torch's own operations."""
+    torch.autograd.graph.increment_version(t)
+
+
 def _wants_grad(tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -339,7 +344,8 @@ def causal_conv(x, weight, bias=None, *, start=None, lengths=None, state=None, s
 
 def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_state=None):
     """`causal_conv` of one token per row: x [batch, channels] -> y [batch, channels].  `state`
-    [batch, width-1, channels] moves up by the token, in place or into `new_state`."""
+    [batch, width-1, channels] moves up by the token, in place or into `new_state`.  (A state that a
+    rollout's backward pass still needs is cloned first, or stepped into a `new_state`.)"""
     (B, D), strides, dev = _first("x", x, 2, "[batch, channels]")
     W = _taps(weight, bias, D, dev)
     if state is None:
@@ -359,6 +365,7 @@ def causal_conv_step(x, state, weight, bias=None, *, start=None, silu=True, new_
         block = _pack_conv(dev, TYPES[x.dtype], B, 1, D, W, 1 if silu else 0, x.data_ptr(), strides[0], 0, weight.data_ptr(),
                            pb, *marks, 0, s, to, y.data_ptr(), y.stride(0), 0, *(0,) * 10)
         _call("auv_causal_conv", block, _lib.SEQ_STEP, dev, scratch=False)
+        _written(state if new_state is None else new_state)
     return y
 
 
@@ -483,7 +490,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_
 def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, start=None,
                         new_state=None):
     """`selective_scan` of one token per row: u, delta, z [batch, channels]; B, C [batch, groups, N];
-    `state` [batch, channels, N] moves on by the token, in place or into `new_state`."""
+    `state` [batch, channels, N] moves on by the token, in place or into `new_state`.  (A state that a
+    rollout's backward pass still needs is cloned first, or stepped into a `new_state`.)"""
     shape, strides, dev = _first("u", u, 2, "[batch, channels]")
     head = _scan_head(u, shape, strides, dev, delta, A, B, C, D, z, delta_bias, start, None, state, delta_softplus, True)
     _no_grad_here("selective_scan_step", (u, delta, state, A, B, C, D, z, delta_bias))
@@ -502,6 +510,7 @@ def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=Non
     if shape[0] and shape[1]:
         block = _pack_scan(*head, to, y.data_ptr(), y.stride(0), 0, *(0,) * 26)
         _call("auv_selective_scan", block, _lib.SEQ_STEP, dev, scratch=False)
+        _written(state if new_state is None else new_state)
     return y
 
 
@@ -662,8 +671,9 @@ class EpisodeMemory(nn.Module):
     `forward(features, start=None, lengths=None, state=None)` takes [batch, length, features]
     and gives ([batch, length, channels], state behind the rows); `step(features, state,
     start=None)` takes [batch, features], gives [batch, channels] and moves `state`
-    (`new_state(batch)`, or one that forward gave) on in place.  Both compute the same
-    function: a rollout stepped token by token and the rollout at once agree to rounding."""
+    (`new_state(batch)`, or one that forward gave) on in place: clone one that a backward
+    pass still needs.  Both compute the same function: a rollout stepped token by token and
+    the rollout at once agree to rounding."""
 
     def __init__(self, features: int, channels: int = 64, layers: int = 1, *, inner: int | None = None, states: int = 16,
                  width: int = 4, dtype=torch.float32):

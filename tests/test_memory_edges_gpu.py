@@ -196,3 +196,45 @@ def test_a_last_token_that_is_not_finite_meets_its_own_taps_only(W, dtype):
     K = W + 2 + 8
     for name, g in (("y", y), ("x", dx), ("weight", dw), ("bias", db)):
         finite_alike(name, g, want[name], 2 * K + W + B * L)
+
+
+# ----------------------------------------------------------------------------
+# calls that other torch machinery makes
+# ----------------------------------------------------------------------------
+def test_a_state_that_was_stepped_on_is_no_good_for_backward_any_more():
+    """A rollout from a state keeps it for its backward pass; a step that moves it on in place is such a change as
+    torch's own in-place operations make, and backward says so."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(37, "float32")
+    B, L, D, N = 2, 5, 8, 4
+    t, _, _ = scan_case(m, B, L, D, N, 1, None, None, True, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    u, w = t["u"].requires_grad_(True), m.par(D, 4)
+    scan = [u] + [t[k] for k in SCAN_ARGS[1:]]
+    token = [v.detach()[:, 0] if v.dim() > 2 else v for v in scan]
+    conv_state, conv_other, scan_state, scan_other = m.rows(B, 3, D), m.rows(B, 3, D), t["state"], m.par(B, D, N)
+    conv = lambda s: memory.causal_conv(u, w, state=s).sum()                                            # noqa: E731
+    rows = lambda s: memory.selective_scan(*scan, state=s).sum()                                        # noqa: E731
+    step_conv = lambda s, to: memory.causal_conv_step(u.detach()[:, 0], s, w, new_state=to)             # noqa: E731
+    step_rows = lambda s, to: memory.selective_scan_step(*token[:2], s, *token[2:], new_state=to)       # noqa: E731
+    for call, step, state, other in ((conv, step_conv, conv_state, conv_other), (rows, step_rows, scan_state, scan_other)):
+        for s, to in ((state, None), (other, other)):        # moved on in place; written as the new state of another
+            y = call(s)
+            before = s._version
+            step(state if to is not None else s, to)
+            assert s._version > before
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+        y = call(state)
+        step(state, other)                                   # the old state is left as it was
+        y.backward()
+    net = memory.EpisodeMemory(6, 8, states=4).cuda()
+    x = torch.randn(B, L, 6, device="cuda")
+    with torch.no_grad():
+        _, s = net(x)
+    h, _ = net(x, state=s)
+    net.step(x[:, 0], s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
