@@ -39,6 +39,7 @@ import weakref
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -144,7 +145,18 @@ def _written(t):
     torch.autograd.graph.increment_version(t)
 
 
+def _no_tangents(tensors):
+    """Forward-mode derivatives end at these calls: refused, for they would end in silence (a tensor with a tangent need not
+    require a gradient)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:        # within a dual_level, as far as this torch tells
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the sequence operators have no forward-mode derivatives")
+
+
 def _wants_grad(tensors):
+    """Whether the call has to be recorded for a backward pass."""
+    _no_tangents(tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

@@ -238,3 +238,40 @@ def test_a_state_that_was_stepped_on_is_no_good_for_backward_any_more():
     net.step(x[:, 0], s)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+def _calls():
+    """Each public call with a first argument of our choice: (name, shape of that argument, call)."""
+    from gym_auv_amd import memory
+
+    m = Maker(38, "float32")
+    B, L, D, N = 2, 5, 8, 4
+    w, wn, A = m.par(D, 4), m.par(D), -m.par(D, N).abs()
+    x, bc = m.rows(B, L, D), m.rows(B, L, 1, N)
+    return [
+        ("causal_conv", (B, L, D), lambda t: memory.causal_conv(t, w)),
+        ("causal_conv weight", (D, 4), lambda t: memory.causal_conv(x, t)),
+        ("causal_conv_step", (B, D), lambda t: memory.causal_conv_step(t, m.rows(B, 3, D), w)),
+        ("selective_scan", (B, L, D), lambda t: memory.selective_scan(t, x, A, bc, bc)),
+        ("selective_scan z", (B, L, D), lambda t: memory.selective_scan(x, x, A, bc, bc, z=t)),
+        ("selective_scan_step", (B, D), lambda t: memory.selective_scan_step(t, x[:, 0], m.par(B, D, N), A, bc[:, 0], bc[:, 0])),
+        ("residual_norm", (B, L, D), lambda t: memory.residual_norm(t, x, wn)),
+        ("residual_norm of rows", (B, D), lambda t: memory.residual_norm(x[:, 0], t, wn)),
+        ("rms_norm", (B, L, D), lambda t: memory.rms_norm(t, wn)),
+        ("rms_norm weight", (D,), lambda t: memory.rms_norm(x, t)),
+    ]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """None of the calls has them; without an error the tangent would be gone in silence."""
+    torch = torch_()
+    import torch.autograd.forward_ad as fwd
+
+    for name, shape, call in _calls():
+        with fwd.dual_level(), torch.set_grad_enabled(grad):
+            call(torch.ones(shape, device="cuda"))                                    # nothing has a tangent: computed
+            dual = fwd.make_dual(torch.ones(shape, device="cuda"), torch.ones(shape, device="cuda"))
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(dual)
+                raise AssertionError(name)
