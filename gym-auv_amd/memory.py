@@ -23,7 +23,8 @@ float32; arithmetic is in 32 bits and every output is rounded once.  Calls run o
 torch's current stream of the tensors' device, never synchronise, and give the same
 bits on every call.  They can be captured into a graph.  A captured backward pass is
 refused while an eager graph of the same parameters is still alive: drop the outputs of
-earlier eager passes first.
+earlier eager passes first.  Forward-mode derivatives and traces (torch.jit.trace,
+make_fx) are refused; torch.compile breaks its graph at these calls and runs them.
 
 `EpisodeMemory` strings them together; `cnn.PerceptionNavigationExtractor(memory=...)`
 steps one behind the scan's features.
@@ -38,9 +39,9 @@ import weakref
 
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -57,8 +58,16 @@ _LEAST = torch.finfo(torch.float32).smallest_normal
 # A call on a single vessel takes the GPU some 3 us, so the host's part counts: each check returns what the call goes on
 # to use, and the argument blocks (include/auvsim.h: 64-bit fields only) are packed in one go.
 
+def _no_trace():
+    """A trace would record the memory for the results, and not the kernels that fill it: outputs that nothing has written
+    whenever it is run."""
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise RuntimeError("the sequence operators cannot be traced: call them outside of the trace")
+
+
 def _first(name, t, dims, what):
     """The tensor that fixes a call's type and device: (shape, strides, device number)."""
+    _no_trace()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:

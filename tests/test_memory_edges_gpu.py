@@ -275,3 +275,34 @@ def test_forward_mode_derivatives_are_refused(grad):
             with pytest.raises(NotImplementedError, match="forward"):
                 call(dual)
                 raise AssertionError(name)
+
+
+def test_tracing_is_refused():
+    """A trace would record the memory for the results and not the kernels that fill it."""
+    torch = torch_()
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for name, shape, call in _calls():
+        x = torch.ones(shape, device="cuda")
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+            raise AssertionError(name)
+        for pre in (False, True):
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(call, pre_dispatch=pre)(x)
+                raise AssertionError(name)
+        call(x)
+
+
+def test_compiled_code_runs_the_calls():
+    """torch.compile cannot look into them: it breaks its graph there, and the results are the eager ones."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m = Maker(39, "float32")
+    x, w = m.rows(2, 5, 8), m.par(8, 4)
+    fn = lambda t: memory.causal_conv(t * 2.0, w) + 1.0          # noqa: E731
+    a, b = (x.clone().requires_grad_(True) for _ in range(2))
+    got, want = torch.compile(fn, backend="eager")(a), fn(b)
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(got.sum(), a)[0], torch.autograd.grad(want.sum(), b)[0])
