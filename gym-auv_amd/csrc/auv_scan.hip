@@ -26,7 +26,7 @@ struct Chunks {
 // backwards: 105 us with chunks for two waves per SIMD and of 32 tokens at least, 71 us for four and of 16.)
 Chunks split(int64_t L, int64_t waves, int64_t enough) {
     constexpr int64_t kTarget = 4096;   // four waves per SIMD
-    if (waves >= enough) return {L, 1};
+    if (waves >= enough || waves == 0 || L == 0) return {L, 1};     // (an empty batch has no waves)
     const int64_t want = ceil_div(kTarget, waves);
     int64_t length = ceil_div(ceil_div(L, want), kSegment) * kSegment;
     const int64_t count = ceil_div(L, length);

@@ -1,8 +1,11 @@
 """The sequence operators at the edges of what they take, as far as no GPU is needed to see it."""
+import ctypes as C
+
 import pytest
 import torch
 
-from gym_auv_amd import memory
+from gym_auv_amd import _lib, memory
+from tests.test_memory_cpu import FAKE, conv_args, norm_args, scan_args
 
 
 def test_tracing_is_refused():
@@ -20,3 +23,17 @@ def test_tracing_is_refused():
                 make_fx(call, pre_dispatch=pre)(x)
         with pytest.raises(ValueError, match="CUDA"):
             call(x)
+
+
+@pytest.mark.parametrize("shape", [dict(batch=0), dict(length=0), dict(batch=0, length=0)], ids=str)
+def test_empty_batches_at_the_c_entry(lib, shape):
+    """A planned launch of nothing: sizes of 0 and, backwards, a refusal, in every pass that takes them."""
+    for fn, args in (("auv_causal_conv", conv_args), ("auv_selective_scan", scan_args), ("auv_residual_norm", norm_args)):
+        a = args(**shape, d_y=FAKE, d_x=FAKE) if fn != "auv_selective_scan" else args(
+            **shape, segments=FAKE, d_y=FAKE, d_u=FAKE, d_delta=FAKE, d_B=FAKE, d_C=FAKE)
+        for what in (_lib.SEQ_FORWARD, _lib.SEQ_BACKWARD):
+            assert getattr(lib, fn + "_workspace")(C.byref(a), what) == 0
+        assert getattr(lib, fn)(C.byref(a), _lib.SEQ_FORWARD, None) == 0
+        assert getattr(lib, fn)(C.byref(a), _lib.SEQ_BACKWARD, None) == -1
+        assert b"empty batch" in lib.auv_seq_last_error()
+    assert lib.auv_selective_scan_segments(C.byref(scan_args(**shape))) == 0
