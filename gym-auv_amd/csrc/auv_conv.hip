@@ -82,8 +82,11 @@ int launch(const auv_conv_args& p, int32_t pass, const Plan& r, ConvArgs a, hipS
     s.n[1] = 1;
     s.dst[0] = p.d_weight;
     s.dst[1] = p.d_bias;
-    hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)ceil_div(s.count, kSumOutputs)), dim3(kSumOutputs * kSumLanes), 0, stream, s);
-    return launched("k_seq_sum");
+    return in_slices(ceil_div(s.count, kSumOutputs), kSumOutputs * kSumLanes, [&](int64_t first, int64_t count) {
+        s.first = first;
+        hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)count), dim3(kSumOutputs * kSumLanes), 0, stream, s);
+        return launched("k_seq_sum");
+    });
 }
 
 template <class T, int W>

@@ -39,11 +39,14 @@ int check(const auv_norm_args& p, int32_t pass) {
 }
 
 template <class TR, class T, int TPR>
-int launch(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t blocks, hipStream_t stream) {
+int launch(const auv_norm_args& p, int32_t pass, NormArgs a, int64_t blocks, hipStream_t stream) {
     constexpr int TH = norm_threads<TPR>();
     if (pass == AUV_SEQ_FORWARD) {
-        hipLaunchKernelGGL((k_norm_forward<TR, T, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
-        return launched("k_norm_forward");
+        return in_slices(blocks, TH, [&](int64_t first, int64_t count) {
+            a.first = first;
+            hipLaunchKernelGGL((k_norm_forward<TR, T, TPR>), dim3((unsigned)count), dim3(TH), 0, stream, a);
+            return launched("k_norm_forward");
+        });
     }
     hipLaunchKernelGGL((k_norm_backward<TR, T, TPR>), dim3((unsigned)blocks), dim3(TH), 0, stream, a);
     if (const int rc = launched("k_norm_backward")) return rc;
@@ -55,8 +58,11 @@ int launch(const auv_norm_args& p, int32_t pass, const NormArgs& a, int64_t bloc
     s.inner = 3;
     s.n[0] = s.n[1] = s.n[2] = 1;
     s.dst[0] = p.d_post_weight, s.dst[1] = p.d_pre_weight, s.dst[2] = p.d_scale;
-    hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)ceil_div(s.count, kSumOutputs)), dim3(kSumOutputs * kSumLanes), 0, stream, s);
-    return launched("k_seq_sum");
+    return in_slices(ceil_div(s.count, kSumOutputs), kSumOutputs * kSumLanes, [&](int64_t first, int64_t count) {
+        s.first = first;
+        hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)count), dim3(kSumOutputs * kSumLanes), 0, stream, s);
+        return launched("k_seq_sum");
+    });
 }
 
 template <class TR, class T>
@@ -108,7 +114,7 @@ int auv_residual_norm(const auv_norm_args* p, int32_t pass, void* stream) {
     const int64_t rows = p->batch * p->length;
     const bool sums = pass == AUV_SEQ_BACKWARD && (p->d_post_weight || p->d_pre_weight || p->d_scale);
     const int64_t blocks = pass == AUV_SEQ_FORWARD ? ceil_div(rows, rows_of(lanes_of(p->channels))) : back_blocks(rows, p->channels);
-    if (blocks > 0x7fffffff) return seq_fail(AUV_ERR_ARG, "auv_residual_norm: too many rows for one launch");
+    if (blocks > 0x7fffffff) return seq_fail(AUV_ERR_ARG, "auv_residual_norm: too many rows");
     if (sums && (!p->workspace || p->workspace_bytes < blocks * p->channels * 3 * (int64_t)sizeof(float)))
         return seq_fail(AUV_ERR_MEMORY, "auv_residual_norm: the workspace holds %lld bytes, too few", (long long)p->workspace_bytes);
     DeviceScope scope(p->device);

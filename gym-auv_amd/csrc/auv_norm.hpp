@@ -32,6 +32,7 @@ struct NormArgs {
     void *dx, *dy, *dgate;
     int64_t dx_row, dx_token, dy_row, dy_token, dgate_row, dgate_token;
     float* partial;          // [gridDim.x, D, 3]: post_weight, pre_weight, scale
+    int64_t first;           // forwards: workgroup of this launch
 };
 
 constexpr int kNormLane = 8;   // elements of a row per lane
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
     __shared__ float buf[2][TH / 64][1];
     const Columns<TPR> me((int)a.D);
     const int d = me.d, slot = threadIdx.x / TPR;
-    const int64_t rows = a.B * a.L, row = (int64_t)blockIdx.x * ROWS + slot, real = row < rows ? row : rows - 1;
+    const int64_t rows = a.B * a.L, row = (a.first + blockIdx.x) * ROWS + slot, real = row < rows ? row : rows - 1;
     const int count = row < rows ? me.mine : 0;
     const int64_t b = real / a.L, l = real - b * a.L;
     const float inv = 1.0f / (float)a.D;

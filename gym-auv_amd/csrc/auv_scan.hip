@@ -9,7 +9,7 @@ namespace auv {
 namespace seq {
 namespace {
 
-constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxGrid = 0x7fffffff;   // waves, numbered in 32 bits, and workgroups, over all launches of a kernel
 
 // States are padded to 4, 8, 16, 32 or 64: lanes per channel of the backward and step kernels, four states each.
 int lanes_of(int64_t states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
@@ -131,14 +131,18 @@ int join(const ScanArgs& a, int NP, bool reverse, hipStream_t stream) {
 
 template <class T, int NPL, int S>
 int run_forward(ScanArgs a, const Forward& f, hipStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(f.waves * f.chunks.count, kScanWaves)), block(kScanWaves * 64);
-    if (f.chunks.count > 1) {
-        hipLaunchKernelGGL((k_scan_forward<T, NPL, S, 1>), grid, block, 0, stream, a);
+    const int64_t blocks = ceil_div(f.waves * f.chunks.count, kScanWaves);
+    const dim3 block(kScanWaves * 64);
+    if (f.chunks.count > 1) {       // (there are few waves then)
+        hipLaunchKernelGGL((k_scan_forward<T, NPL, S, 1>), dim3((unsigned)blocks), block, 0, stream, a);
         if (const int rc = launched("k_scan_forward")) return rc;
         if (const int rc = join(a, NPL * S, false, stream)) return rc;
     }
-    hipLaunchKernelGGL((k_scan_forward<T, NPL, S, 0>), grid, block, 0, stream, a);
-    return launched("k_scan_forward");
+    return in_slices(blocks, kScanWaves * 64, [&](int64_t first, int64_t count) {
+        a.first = first;
+        hipLaunchKernelGGL((k_scan_forward<T, NPL, S, 0>), dim3((unsigned)count), block, 0, stream, a);
+        return launched("k_scan_forward");
+    });
 }
 
 template <class T, int S, bool TAIL>
@@ -166,9 +170,12 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
     hipLaunchKernelGGL((k_scan_backward<T, S, 0, TAIL>), grid, block, lds, stream, a);
     if (const int rc = launched("k_scan_backward")) return rc;
     if (a.bc_partial) {
-        const int64_t n = ceil_div(a.B * a.L * a.G * 2 * 4 * S, 256);
-        hipLaunchKernelGGL((k_scan_sum_bc<T>), dim3((unsigned)n), dim3(256), 0, stream, a, 4 * S, (int)r.blocks);
-        if (const int rc = launched("k_scan_sum_bc")) return rc;
+        const int rc = in_slices(ceil_div(a.B * a.L * a.G * 2 * 4 * S, 256), 256, [&](int64_t first, int64_t count) {
+            a.first = first;
+            hipLaunchKernelGGL((k_scan_sum_bc<T>), dim3((unsigned)count), dim3(256), 0, stream, a, 4 * S, (int)r.blocks);
+            return launched("k_scan_sum_bc");
+        });
+        if (rc) return rc;
     }
     SumArgs s{};
     s.src = a.partial;
@@ -177,8 +184,11 @@ int run_backward(ScanArgs a, const auv_scan_args& p, const Backward& r, hipStrea
     s.inner = a.N + 2;
     s.n[0] = a.N, s.n[1] = s.n[2] = 1;
     s.dst[0] = p.d_A, s.dst[1] = p.d_D, s.dst[2] = p.d_delta_bias;
-    hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)ceil_div(s.count, kSumOutputs)), dim3(kSumOutputs * kSumLanes), 0, stream, s);
-    return launched("k_seq_sum");
+    return in_slices(ceil_div(s.count, kSumOutputs), kSumOutputs * kSumLanes, [&](int64_t first, int64_t count) {
+        s.first = first;
+        hipLaunchKernelGGL(k_seq_sum, dim3((unsigned)count), dim3(kSumOutputs * kSumLanes), 0, stream, s);
+        return launched("k_seq_sum");
+    });
 }
 
 template <class T, int S>
@@ -271,7 +281,7 @@ int launches_fit(const auv_scan_args& p, int32_t pass) {
         const Backward r = backward_plan(p);
         if (r.bc_bytes && ceil_div(p.batch * p.length * p.groups * 8 * S, 256) > kMaxGrid) most = kMaxGrid + 1;
     }
-    return most > kMaxGrid ? seq_fail(AUV_ERR_ARG, "auv_selective_scan: batch too large for one launch") : AUV_OK;
+    return most > kMaxGrid ? seq_fail(AUV_ERR_ARG, "auv_selective_scan: batch too large") : AUV_OK;
 }
 }  // namespace
 }  // namespace seq

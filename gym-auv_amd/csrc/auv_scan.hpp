@@ -57,6 +57,7 @@ struct ScanArgs {
     int32_t lanes;           // threads side by side on a row's channels in a step
     int32_t whole;           // rows of activations and of their gradients may be read and written in fours
     float* bc_partial;       // [tile blocks, B, L, G, 2, NP] when a group's channels fill more than one workgroup
+    int64_t first;           // forwards and in k_scan_sum_bc: workgroup of this launch
 };
 
 __device__ __forceinline__ void wave_sync() {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kScanWaves * 64) void k_scan_forward(ScanArgs a) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int q = lane % S, c = lane / S;
     const int Dg = (int)(a.D / a.G), tiles = (Dg + CW - 1) / CW;
-    unsigned id = blockIdx.x * kScanWaves + wave;             // the host sees to it that there are fewer than 2^31
+    unsigned id = ((unsigned)a.first + blockIdx.x) * kScanWaves + wave;             // the host sees to it that there are fewer than 2^31
     const int ct = id % tiles;
     id /= tiles;
     const int g = id % (unsigned)a.G;
@@ -811,7 +812,7 @@ __global__ __launch_bounds__(scan_back_waves<S>() * 64, S == 4 ? 4 : S == 8 ? 3 
 template <class T>
 __global__ __launch_bounds__(256) void k_scan_sum_bc(ScanArgs a, int NP, int blocks) {
     const int64_t count = a.B * a.L * a.G * 2 * NP;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (a.first + blockIdx.x) * 256 + threadIdx.x;
     if (i >= count) return;
     const int s = (int)(i % NP), which = (int)(i / NP % 2);
     const int64_t g = i / (2 * NP) % a.G, t = i / (2 * NP * a.G) % a.L, b = i / (2 * NP * a.G * a.L);

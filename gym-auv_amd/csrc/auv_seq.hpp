@@ -311,11 +311,12 @@ struct SumArgs {
     int32_t inner;
     int32_t n[3];
     float* dst[3];
+    int64_t first;          // workgroup of this launch
 };
 static __global__ __launch_bounds__(kSumOutputs * kSumLanes) void k_seq_sum(SumArgs a) {
     __shared__ float part[kSumLanes][kSumOutputs + 1];
     const int o = threadIdx.x % kSumOutputs, s0 = threadIdx.x / kSumOutputs;
-    const int64_t m = (int64_t)blockIdx.x * kSumOutputs + o;
+    const int64_t m = (a.first + blockIdx.x) * kSumOutputs + o;
     float acc = 0.0f;
     if (m < a.count) {
 #pragma unroll 8

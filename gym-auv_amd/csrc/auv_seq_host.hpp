@@ -3,6 +3,7 @@
 #pragma once
 
 #include "../../include/auvsim.h"
+#include "auv_slices.hpp"
 
 #include <hip/hip_runtime.h>
 

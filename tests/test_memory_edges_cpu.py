@@ -37,3 +37,19 @@ def test_empty_batches_at_the_c_entry(lib, shape):
         assert getattr(lib, fn)(C.byref(a), _lib.SEQ_BACKWARD, None) == -1
         assert b"empty batch" in lib.auv_seq_last_error()
     assert lib.auv_selective_scan_segments(C.byref(scan_args(**shape))) == 0
+
+
+def test_launches_stay_within_a_grid(tmp_path):
+    """The spread of workgroups over launches (csrc/auv_slices.hpp), built for the host and checked there."""
+    import os
+    import shutil
+    import subprocess
+
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "slices_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-I", os.path.join(root, "gym-auv_amd", "csrc"), "-o", exe,
+                    os.path.join(root, "tests", "native", "slices_check.cpp")], check=True)
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and run.stdout.startswith("slices ok"), run.stdout + run.stderr

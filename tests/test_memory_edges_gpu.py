@@ -306,3 +306,69 @@ def test_compiled_code_runs_the_calls():
     got, want = torch.compile(fn, backend="eager")(a), fn(b)
     assert torch.equal(got, want)
     assert torch.equal(torch.autograd.grad(got.sum(), a)[0], torch.autograd.grad(want.sum(), b)[0])
+
+
+# ----------------------------------------------------------------------------
+# sizes beyond one launch
+# ----------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,D", [(4_194_303 + 70, 2056), (16_777_215 + 90, 520), ((1 << 30) + 130, 4)])
+def test_norm_of_more_rows_than_one_launch_takes(rows, D):
+    """A row takes a workgroup of 1,024 or 256 threads, or a 64th of one: 2^32 threads and more."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    torch.manual_seed(8)
+    x = torch.zeros(rows, D, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(D, device="cuda")
+    at = [0, rows - 131, rows - 100, rows - 71, rows - 70, rows - 69, rows - 5, rows - 1]
+    at = torch.tensor([i for i in at if 0 <= i], device="cuda")
+    x[at] = torch.randn(len(at), D, device="cuda").bfloat16()
+    h = memory.rms_norm(x, w)
+    assert torch.equal(h[at], memory.rms_norm(x[at], w))
+    assert int(torch.count_nonzero(h[-200:].any(1))) == len(at) - 1 and not h[1:1000].any()
+
+
+def test_scan_of_more_waves_than_one_launch_takes():
+    """A group of one channel takes a wave of its own: 2^26 of them and more."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    torch.manual_seed(9)
+    B, D = (1 << 20) + 33, 64
+    u, delta, bc = torch.zeros(B, 1, D, device="cuda"), torch.zeros(B, 1, D, device="cuda"), torch.zeros(B, 1, D, 1, device="cuda")
+    at = torch.tensor([0, 1, (1 << 20) - 2, (1 << 20) - 1, 1 << 20, B - 1], device="cuda")
+    for t in (u, delta, bc):
+        t[at] = torch.randn(t[at].shape, device="cuda")
+    A = -torch.rand(D, 1, device="cuda")
+    y, h = memory.selective_scan(u, delta, A, bc, bc, return_state=True)
+    few = [t[at] for t in (u, delta, bc)]
+    # (few rows take another form of the kernel where a channel has more than 4 states: not here)
+    ys, hs = memory.selective_scan(few[0], few[1], A, few[2], few[2], return_state=True)
+    assert torch.equal(y[at], ys) and torch.equal(h[at], hs)
+    assert int(torch.count_nonzero(y.any(2))) == len(at)
+
+
+def test_scan_gradients_of_more_sums_than_one_launch_takes():
+    """dB and dC of a group wider than a workgroup are summed over its workgroups by a launch of their own: 2^32 numbers."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    torch.manual_seed(10)
+    B, L, D, N, bf = (1 << 18) + 5, 128, 32, 64, torch.bfloat16
+    at = torch.tensor([0, (1 << 18) - 1, 1 << 18, B - 1], device="cuda")
+    rows = lambda *tail: torch.zeros(B, L, *tail, device="cuda", dtype=bf)          # noqa: E731
+    u, delta, Bm, Cm, gy = rows(D), rows(D), rows(1, N), rows(1, N), rows(D)
+    for t in (u, delta, Bm, Cm, gy):
+        t[at] = torch.randn(len(at), *t.shape[1:], device="cuda").to(bf)
+    A = -torch.rand(D, N, device="cuda")
+    few = [t[at].requires_grad_(True) for t in (u, delta, Bm, Cm)]
+    Bm.requires_grad_(True), Cm.requires_grad_(True)
+    y = memory.selective_scan(u, delta, A, Bm, Cm)
+    dB, dC = torch.autograd.grad(y, [Bm, Cm], gy)
+    ys = memory.selective_scan(few[0], few[1], A, few[2], few[3])
+    wB, wC = torch.autograd.grad(ys, few[2:], gy[at])
+    assert torch.equal(y.detach()[at], ys.detach()) or float((y.detach()[at].float() - ys.detach().float()).abs().max()) <= 2 ** -7 * float(ys.detach().float().abs().max())
+    for got, want in ((dB, wB), (dC, wC)):
+        # a few rows are split over time: other orders of the same sums, then one rounding to bfloat16, half a step (2^-8) each
+        assert float((got[at].float() - want.float()).abs().max()) <= 2 ** -7 * float(want.float().abs().max())
+        assert not got[1:1000].any() and int(torch.count_nonzero(got[-100:].flatten(1).any(1))) == 3
