@@ -690,7 +690,8 @@ class EpisodeMemory(nn.Module):
     `layers` blocks of convolution and scan between gated norms, and a last norm.
 
     `forward(features, start=None, lengths=None, state=None)` takes [batch, length, features]
-    and gives ([batch, length, channels], state behind the rows); `step(features, state,
+    and gives ([batch, length, channels], state behind the rows), zeros behind each row's
+    last token (`lengths`); `step(features, state,
     start=None)` takes [batch, features], gives [batch, channels] and moves `state`
     (`new_state(batch)`, or one that forward gave) on in place: clone one that a backward
     pass still needs.  Both compute the same function: a rollout stepped token by token and
@@ -741,8 +742,14 @@ class EpisodeMemory(nn.Module):
                 return y
             return conv, scan
 
+        real = None
+        if lengths is not None:
+            # the layers between the operators know no lengths: what lies behind a row's last token goes in as zeros, so that
+            # no gradient of a parameter sees it, and comes out as zeros
+            real = (torch.arange(features.shape[1], device=features.device) < lengths[:, None])[..., None]
+            features = torch.where(real, features, 0)
         h = self._run(features, [mixer(layer, None if state is None else state[i]) for i, layer in enumerate(self.layers)])
-        return h, [tuple(s) for s in out]
+        return h if real is None else torch.where(real, h, 0), [tuple(s) for s in out]
 
     @torch.no_grad()
     def step(self, features, state, start=None):

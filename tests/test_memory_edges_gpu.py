@@ -372,3 +372,41 @@ def test_scan_gradients_of_more_sums_than_one_launch_takes():
         # a few rows are split over time: other orders of the same sums, then one rounding to bfloat16, half a step (2^-8) each
         assert float((got[at].float() - want.float()).abs().max()) <= 2 ** -7 * float(want.float().abs().max())
         assert not got[1:1000].any() and int(torch.count_nonzero(got[-100:].flatten(1).any(1))) == 3
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_memory_of_padded_rows(dtype):
+    """What lies behind a row's last token, NaN and infinities included, has no part in outputs, states and gradients; the
+    outputs there are 0."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    torch.manual_seed(6)
+    B, L, F = 4, 21, 18
+    net = memory.EpisodeMemory(F, 16, layers=2, dtype=getattr(torch, dtype)).cuda()
+    x = torch.randn(B, L, F, device="cuda")
+    n = torch.tensor([L, 0, 7, 16], dtype=torch.int32, device="cuda")
+    weight = torch.randn(B, L, 16, device="cuda")
+    params = list(net.parameters())
+
+    def run(fill):
+        v = x.clone()
+        for b, k in enumerate(n.tolist()):
+            v[b, k:] = fill
+        v.requires_grad_(True)
+        h, state = net(v, lengths=n)
+        return h.detach(), [t.detach() for s in state for t in s], torch.autograd.grad((h.float() * weight).sum(), [v] + params)
+
+    h0, s0, g0 = run(0.0)
+    assert all(bool(torch.isfinite(g).all()) for g in g0)
+    for b, k in enumerate(n.tolist()):
+        assert not h0[b, k:].any() and not g0[0][b, k:].any()
+        if k:        # and the row is the row by itself
+            alone, s = net(x[b:b + 1, :k])
+            tol = (2e-5 if dtype == "float32" else 0.08) * float(alone.float().abs().max())
+            assert float((alone - h0[b:b + 1, :k]).float().abs().max()) <= tol
+    for fill in (float("nan"), float("inf")):
+        h1, s1, g1 = run(fill)
+        assert torch.equal(h0, h1)
+        for a, c in zip(s0 + list(g0), s1 + list(g1)):
+            assert torch.equal(a, c)
