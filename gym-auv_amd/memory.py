@@ -695,7 +695,7 @@ class EpisodeMemory(nn.Module):
     start=None)` takes [batch, features], gives [batch, channels] and moves `state`
     (`new_state(batch)`, or one that forward gave) on in place: clone one that a backward
     pass still needs.  Both compute the same function: a rollout stepped token by token and
-    the rollout at once agree to rounding."""
+    the rollout at once agree to rounding.  Types are those of `dtype` under torch.autocast too."""
 
     def __init__(self, features: int, channels: int = 64, layers: int = 1, *, inner: int | None = None, states: int = 16,
                  width: int = 4, dtype=torch.float32):
@@ -717,6 +717,9 @@ class EpisodeMemory(nn.Module):
                  torch.zeros(batch, self.inner, self.states, device=dev)) for _ in self.layers]
 
     def _run(self, features, mixers):
+        if torch.is_autocast_enabled():                # the types are the module's own
+            with torch.autocast("cuda", enabled=False):
+                return self._run(features.to(self.enter.weight.dtype), mixers)
         x = self.enter(features)                       # the residual stream, in 32 bits
         h = rms_norm(x, self.layers[0].pre_weight, dtype=self.dtype)
         for i, (layer, (conv, scan)) in enumerate(zip(self.layers, mixers)):

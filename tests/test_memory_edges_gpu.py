@@ -410,3 +410,26 @@ def test_memory_of_padded_rows(dtype):
         assert torch.equal(h0, h1)
         for a, c in zip(s0 + list(g0), s1 + list(g1)):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("under", ["bfloat16", "float16"])
+def test_memory_under_autocast_keeps_its_own_types(dtype, under):
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    torch.manual_seed(7)
+    net = memory.EpisodeMemory(18, 16, layers=2, dtype=getattr(torch, dtype)).cuda()
+    x = torch.randn(3, 9, 18, device="cuda")
+    want, _ = net(x)
+    got_state, want_state = net.new_state(3), net.new_state(3)
+    wants = net.step(x[:, 0], want_state)
+    with torch.autocast("cuda", dtype=getattr(torch, under)):
+        got, _ = net(x)
+        gots = net.step(x[:, 0], got_state)
+        low, _ = net(x.to(getattr(torch, under)))          # what an autocast layer in front hands over
+        assert torch.is_autocast_enabled()
+    assert got.dtype == want.dtype and torch.equal(got, want) and torch.equal(gots, wants)
+    assert low.dtype == want.dtype and bool(torch.isfinite(low).all())
+    g0, g1 = torch.autograd.grad(want.sum(), net.enter.weight), torch.autograd.grad(got.sum(), net.enter.weight)
+    assert torch.equal(g0[0], g1[0])
