@@ -117,7 +117,11 @@ class PerceptionNavigationExtractor:
     one token of every env's episode and returns the memory's features instead;
     `start` (B,) marks the envs whose episode begins with this observation
     (`sim.tensor("t_step") == 0`).  The state of the batch is kept between
-    calls; `reset()` forgets it."""
+    calls and moved on in place; `reset()` forgets it.
+
+    A call is `remember(tokens(obs), start)`.  A rollout that the memory is
+    trained on keeps the tokens and starts of its steps, and clones of the
+    tensors in `state` from before the first, unless that opens an episode."""
 
     def __init__(self, kind: str, state_dict, device: int = 0, memory=None):
         self.cnn = LidarCNN(kind, state_dict, device)
@@ -128,19 +132,32 @@ class PerceptionNavigationExtractor:
             raise ValueError(f"the memory takes {memory.features} features, the extractor has {width}")
         self.features_dim = width if memory is None else memory.channels
 
+    @property
+    def state(self):
+        """The memory's state of the batch, (convolution, scan) per layer; None before an episode's first call."""
+        return self._state
+
     def reset(self):
         self._state = None
 
-    def __call__(self, obs, start=None):
+    def tokens(self, obs):
+        """Scan features and navigation of each env: what the memory takes."""
         import torch
 
         per = self.cnn.forward(obs["perception"], "features")
         nav = obs["navigation"][:, 0, :]
-        out = torch.cat([per, nav], dim=1)
+        return torch.cat([per, nav], dim=1)
+
+    def remember(self, tokens, start=None):
+        """The memory's features of one token per env; its state moves on."""
         if self.memory is None:
-            if start is not None:
-                raise ValueError("start marks episodes for a memory; this extractor has none")
-            return out
+            raise ValueError("this extractor has no memory")
         if self._state is None:
-            self._state = self.memory.new_state(len(out))
-        return self.memory.step(out, self._state, start)
+            self._state = self.memory.new_state(len(tokens))
+        return self.memory.step(tokens, self._state, start)
+
+    def __call__(self, obs, start=None):
+        if self.memory is None and start is not None:
+            raise ValueError("start marks episodes for a memory; this extractor has none")
+        out = self.tokens(obs)
+        return out if self.memory is None else self.remember(out, start)

@@ -433,3 +433,51 @@ def test_memory_under_autocast_keeps_its_own_types(dtype, under):
     assert low.dtype == want.dtype and bool(torch.isfinite(low).all())
     g0, g1 = torch.autograd.grad(want.sum(), net.enter.weight), torch.autograd.grad(got.sum(), net.enter.weight)
     assert torch.equal(g0[0], g1[0])
+
+
+# ----------------------------------------------------------------------------
+# the extractor's tokens
+# ----------------------------------------------------------------------------
+def test_the_extractor_hands_out_what_its_memory_is_trained_on():
+    """Two rollouts of one batch, the second in the middle of episodes: the memory over the kept tokens, from the state
+    kept before, gives the features that the policy saw, and gradients."""
+    import os
+
+    torch = torch_()
+    from gym_auv_amd import cnn, memory, scenarios
+    from gym_auv_amd.env import VecAuvEnv
+    from oracle import cnn_oracle
+
+    gold = np.load(os.path.join(os.path.dirname(__file__), "golden", "cnn_golden.npz"))
+    cfg, scene = scenarios.make_workload("cfg3_65536_moving", n_envs=64)
+    cfg["max_steps"] = 9
+    env = VecAuvEnv(cfg, scene, auto_reset="device")
+    torch.manual_seed(11)
+    net = memory.EpisodeMemory(18, 16, layers=2).cuda()
+    weights = cnn_oracle.golden_weights(gold, "shallow")
+    ext, whole = (cnn.PerceptionNavigationExtractor("shallow", weights, memory=net) for _ in range(2))
+    assert ext.state is None
+    obs, acts = env.reset(), torch.from_numpy(scenarios.random_actions(64, 20, seed=2)).cuda()
+    for first, steps in ((0, 6), (6, 14)):
+        tokens, starts = torch.zeros(steps, 64, 18, device="cuda"), torch.zeros(steps, 64, dtype=torch.bool, device="cuda")
+        before = None if ext.state is None else [tuple(t.clone() for t in s) for s in ext.state]
+        seen = []
+        for k in range(steps):
+            starts[k] = env.sim.tensor("t_step") == 0
+            tokens[k] = ext.tokens(obs)
+            seen.append(ext.remember(tokens[k], starts[k]))
+            assert torch.equal(seen[-1], whole(obs, starts[k]))
+            obs, _, _, _ = env.step(acts[first + k].t())
+        h, _ = net(tokens.transpose(0, 1), start=starts.transpose(0, 1), state=before)
+        seen = torch.stack(seen, 1)
+        assert float((h - seen).abs().max()) <= 2e-5 * float(seen.abs().max())
+        grads = torch.autograd.grad(h.square().sum(), list(net.parameters()))
+        assert all(bool(torch.isfinite(g).all()) and bool(g.any()) for g in grads)
+    assert starts.any() and not starts[0].all()
+    plain = cnn.PerceptionNavigationExtractor("shallow", weights)
+    assert torch.equal(plain(obs), ext.tokens(obs))
+    with pytest.raises(ValueError, match="no memory"):
+        plain.remember(tokens[0])
+    with pytest.raises(ValueError, match="none"):
+        plain(obs, starts[0])
+    env.close()
