@@ -481,3 +481,75 @@ def test_the_extractor_hands_out_what_its_memory_is_trained_on():
     with pytest.raises(ValueError, match="none"):
         plain(obs, starts[0])
     env.close()
+
+
+# ----------------------------------------------------------------------------
+# many rows a workgroup: sums carried from one to the next
+# ----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,residual", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("B,L,D", [(531, 131, 18), (251, 37, 250), (101, 13, 600), (67, 11, 2050)])
+def test_norm_gradients_of_many_rows_a_workgroup(B, L, D, dtype, residual):
+    """512 workgroups (256 above 2,048 channels) of 64, 8, 1 and 1 rows each go two to three times over; the last time not
+    all of them.  A column's sum goes through its thread's rows, a workgroup's threads and 16 records in each of 32 parts."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    m, r = Maker(40, dtype, "time"), Maker(41, residual, "time")
+    at_once = {18: 64 * 512, 250: 8 * 512, 600: 512, 2050: 256}[D]
+    assert 2 * at_once < B * L < 4 * at_once and B * L % at_once
+    named = dict(x=r.rows(B, L, D), y=m.rows(B, L, D), post_weight=m.par(D), pre_weight=m.par(D), gate=m.rows(B, L, D), scale=m.par(D))
+    named = {k: v.requires_grad_(True) for k, v in named.items()}
+    gx, gh = r.rows(B, L, D), m.rows(B, L, D)
+    outs = memory.residual_norm(*named.values())
+    grads = torch.autograd.grad(outs, list(named.values()), [gx, gh])
+    flat = lambda t: host(t).reshape(-1, D) if t.dim() == 3 else host(t)     # noqa: E731
+    want = O.norm(*(flat(t) for t in named.values()), dx_out=flat(gx), dh=flat(gh))
+    K = 4 * (D + 24) + 4 + 64 + 16 + 32
+    for (name, leaf), g in zip(named.items(), grads):
+        check("d_" + name, g, tuple(v.reshape(leaf.shape) for v in want[name]), K)
+
+
+@pytest.mark.parametrize("B,L,D,W,dtype", [(300, 20, 2100, 4, "float32"), (200, 23, 4100, 3, "bfloat16"), (2100, 20, 520, 4, "float16"),
+                                           (2100, 20, 260, 2, "float32")])
+def test_conv_gradients_of_many_runs_a_thread(B, L, D, W, dtype):
+    """More runs than the records of a backward pass have threads for: a thread goes over several, from row to row."""
+    torch = torch_()
+    from gym_auv_amd import memory
+
+    V = 4 if dtype == "float32" else 8
+    slots = 256 // min(256, -(-D // V))
+    assert B * -(-L // 8) > min(2048, 2 ** 20 // D) * slots
+    m = Maker(42, dtype, "time")
+    start, n = m.starts(B, L, 0.1), lengths_of("ragged", B, L, m.rng)
+    x, w, b = m.rows(B, L, D), m.par(D, W), m.par(D)
+    m.layout = "rows"
+    s = m.rows(B, W - 1, D)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, s)]
+    gy, gs = m.rows(B, L, D), m.rows(B, W - 1, D)
+    y, new = memory.causal_conv(x, w, b, start=start, lengths=n, state=s, return_state=True)
+    grads = torch.autograd.grad([y, new], leaves, [gy, gs])
+    want = O.conv(host(x), host(w), host(b), hostb(start), n.cpu().numpy(), host(s), True, host(gy), host(gs))
+    # a sum goes through a thread's runs of 8 tokens, a workgroup's threads and 64 records in each of 32 parts
+    K = 2 * (W + 10) + W + 8 * 4 + slots + 64 + 32
+    for name, g in zip(("x", "weight", "bias", "state"), grads):
+        check("d_" + name, g, want[name], K)
+
+
+@pytest.mark.parametrize("B,D,N,G,dtype", [(4200, 64, 16, 1, "float32"), (4200, 64, 16, 1, "bfloat16"), (4200, 40, 4, 2, "float16"), (4200, 64, 8, 1, "bfloat16"),
+                                           (2100, 40, 20, 1, "float32"), (1100, 24, 64, 1, "bfloat16")])
+def test_scan_gradients_of_many_rows_a_workgroup(B, D, N, G, dtype):
+    """More rows than the workgroups of a backward pass take at once: sums of A, D and delta_bias carried from row to row."""
+    torch = torch_()
+    L = 5
+    m = Maker(43, dtype, "time")
+    t, start, n = scan_case(m, B, L, D, N, G, 0.2, "ragged", True, True)
+    t = {k: None if v is None else v.detach() for k, v in t.items()}
+    for k in ("u", "delta", "B", "C", "z"):                # (what the padding may hold is not at stake here)
+        t[k] = torch.nan_to_num(t[k], nan=0.0, posinf=0.0)
+    gy, gs = m.rows(B, L, D), m.par(B, D, N)
+    got, want = run_scan(t, start, n, gy, gs, True), raw_scan(t, start, n, gy, gs, True)
+    K = 10 * (L + N + 12)
+    for name in got:
+        # a thread's tokens of up to five rows, then 64 records in each of 32 parts; dB and dC: a group's channels
+        more = 25 + 64 + 32 if name in ("A", "D", "delta_bias") else D // G if name in ("B", "C") else 0
+        check("d_" + name, got[name], want[name], 2 * K + more)
