@@ -122,9 +122,10 @@ int join(const ScanArgs& a, int NP, bool reverse, hipStream_t stream) {
     j.last = reverse ? a.dstate : nullptr;
     j.chunks = a.chunks, j.count = a.B * a.D * NP;
     j.N = a.N, j.NP = NP, j.reverse = reverse;
-    // a workgroup of 64 numbers for each of the 256 CUs, or of 16 where there are fewer and chunks enough for four in each of
-    // its 64 rows: 2,048 numbers of 315 chunks 8.1 us, 10.0 us in 64s; 5,040 of 63 chunks 6.3 us, 4.8 us in 64s
-    if (j.count < 64 * 256 && j.chunks >= 4 * 64) hipLaunchKernelGGL(k_scan_join<16>, dim3((unsigned)ceil_div(j.count, 16)), dim3(kJoinThreads), 0, stream, j);
+    // 64 numbers a workgroup, or 16 where they are few and the chunks enough for four in each of its 64 rows.  Whole forward
+    // passes of 315 chunks: 1,024 numbers 29.1 us in 16s and 35.8 in 64s, 2,048 numbers 35.3 and 36.3; of 256 chunks: 512
+    // numbers 23.2 and 29.2, 4,096 numbers 33.6 and 31.9, 8,192 numbers 59.2 and 54.9; of 63 chunks: 5,040 numbers 24.5 and 21.4
+    if (j.count < 4096 && j.chunks >= 4 * 64) hipLaunchKernelGGL(k_scan_join<16>, dim3((unsigned)ceil_div(j.count, 16)), dim3(kJoinThreads), 0, stream, j);
     else hipLaunchKernelGGL(k_scan_join<64>, dim3((unsigned)ceil_div(j.count, 64)), dim3(kJoinThreads), 0, stream, j);
     return launched("k_scan_join");
 }
