@@ -291,27 +291,27 @@ __global__ __launch_bounds__(kJoinThreads) void k_scan_join(JoinArgs a) {
     auto at = [&](int64_t c) { return (a.reverse ? a.chunks - 1 - c : c) * a.count + i; };
     // s + 2^p x.  Behind a start whatever came before (also an infinity or NaN) has no part in what follows.  Everywhere else
     // it has one: 2^p is multiplied in by halves within [2^-126, 2^127], so that an infinity or NaN stays one however small the
-    // decay, a 0 stays 0 however large, and what is cut off at either end is off by less than 2^-124, or beyond 2^128 too.
-    auto join = [](float p, float x, float s) {
-        const float r = exp2_hw(__builtin_amdgcn_fmed3f(0.5f * p, -126.0f, 127.0f));
-        return p == kCut ? s : fmaf(x * r, r, s);
-    };
+    // decay, a 0 stays 0 however large, and what is cut off at either end is off by less than 2^-124, or beyond 2^128 too.  No
+    // half is 0, which therefore stands for a start.
+    auto half = [](float p) { return p == kCut ? 0.0f : exp2_hw(__builtin_amdgcn_fmed3f(0.5f * p, -126.0f, 127.0f)); };
+    auto join = [](float half, float x, float s) { return half == 0.0f ? s : fmaf(x * half, half, s); };
     float h = 0.0f, p = 0.0f;
     if (live) {
 #pragma unroll 4
         for (int64_t c = c0; c < c1; ++c) {
             const float s = a.chunk_state[at(c)], q = a.chunk_decay[at(c)];
-            h = join(q, h, s);
+            h = join(half(q), h, s);
             p += q;
         }
     }
     hs[row][lane] = h;
-    ps[row][lane] = p;
+    ps[row][lane] = half(p);
     __syncthreads();
     if (!live) return;
     const int64_t bd = i / a.NP;
     const int s = (int)(i - bd * a.NP);
     float x = a.first && s < a.N ? a.first[bd * a.N + s] : 0.0f;
+#pragma unroll 8
     for (int r = 0; r < row; ++r) x = join(ps[r][lane], x, hs[r][lane]);
     for (int64_t c = c0; c < c1; c += 4) {      // four at a time: no load waits behind the stores before it
         float e[4], q[4];
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_scan_join(JoinArgs a) {
         for (int k = 0; k < 4; ++k)
             if (c + k < c1) {
                 a.chunk_state[at(c + k)] = x;
-                x = join(q[k], x, e[k]);
+                x = join(half(q[k]), x, e[k]);
             }
     }
     if (a.last && s < a.N && row == ROWS - 1) a.last[bd * a.N + s] = x;
