@@ -58,16 +58,28 @@ _LEAST = torch.finfo(torch.float32).smallest_normal
 # A call on a single vessel takes the GPU some 3 us, so the host's part counts: each check returns what the call goes on
 # to use, and the argument blocks (include/auvsim.h: 64-bit fields only) are packed in one go.
 
+# What torch tells of itself, by its own shortest ways where this torch has them: a step of one vessel is host time.
+_jit_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_increment_version = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+try:
+    _modes = torch._C._len_torch_dispatch_stack
+    _modes_before_dispatch = torch._ops.mode_stack_state_for_pre_dispatch().get      # of 0: a proxy mode
+    _modes(), _modes_before_dispatch(0)
+except (AttributeError, TypeError):
+    _modes = _modes_before_dispatch = lambda *_: True
+
+
 def _no_trace():
     """A trace would record the memory for the results, and not the kernels that fill it: outputs that nothing has written
     whenever it is run."""
-    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+    if _jit_tracing() or get_proxy_mode() is not None:
         raise RuntimeError("the sequence operators cannot be traced: call them outside of the trace")
 
 
 def _first(name, t, dims, what):
     """The tensor that fixes a call's type and device: (shape, strides, device number)."""
-    _no_trace()
+    if _jit_tracing() or _modes() or _modes_before_dispatch(0):
+        _no_trace()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
@@ -151,21 +163,21 @@ def _in_place(name, lo, t, others):
 
 def _written(t):
     """A kernel has written t: a graph that keeps t for its backward pass has to know, as after torch's own operations."""
-    torch.autograd.graph.increment_version(t)
+    _increment_version((t,))
 
 
 def _no_tangents(tensors):
     """Forward-mode derivatives end at these calls: refused, for they would end in silence (a tensor with a tangent need not
     require a gradient)."""
-    if getattr(forward_ad, "_current_level", 0) >= 0:        # within a dual_level, as far as this torch tells
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("the sequence operators have no forward-mode derivatives")
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the sequence operators have no forward-mode derivatives")
 
 
 def _wants_grad(tensors):
     """Whether the call has to be recorded for a backward pass."""
-    _no_tangents(tensors)
+    if getattr(forward_ad, "_current_level", 0) >= 0:        # within a dual_level, as far as this torch tells
+        _no_tangents(tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
