@@ -10,8 +10,8 @@ thread_local char g_seq_error[512];
 
 // Tokens per thread.  A run re-reads the W - 1 tokens before it, so long runs read less; short ones give a small batch
 // more threads.  Runs of 32 wherever that leaves two waves per SIMD of the 256 CUs (131,072 threads), down to 8.  4,096
-// rows x 128 tokens x 128 channels, bf16, forwards and backwards: 172 us in runs of 32, 229 us in runs of 8; 5 rows of up
-// to 4,001 tokens x 90 channels forwards, with the launch: 25 us and 16 us.
+// rows x 128 tokens x 128 channels, bf16, forwards and backwards: 167 us in runs of 32, 190 in runs of 16, 214 in runs of 8
+// (156 in runs of 64); 5 rows of up to 4,001 tokens x 90 channels forwards: 15.7, 9.8 and 7.0 us.
 int conv_run(int64_t B, int64_t L, int64_t vectors) {
     int run = 32;
     while (run > 8 && B * ceil_div(L, run) * vectors < 131072) run /= 2;
@@ -41,8 +41,8 @@ Plan conv_plan(const auv_conv_args& p, int32_t pass) {
     const int64_t slots = kConvThreads / r.lanes;
     const int64_t want = ceil_div(p.batch * ceil_div(p.length, r.run), slots);
     // forwards: a workgroup per set of runs; backwards a workgroup takes several, because each leaves a record of sums;
-    // a step's takes several rows, because it loads its taps first (65,536 rows of 128 channels, with the launch: 34 us, 37
-    // us with a workgroup for every 16 rows)
+    // a step's takes several rows, because it loads its taps first (65,536 rows of 128 channels: 23.8 us, 25.1 us with a
+    // workgroup for every 16 rows)
     const int64_t cap = pass == AUV_SEQ_BACKWARD ? conv_records(p.channels) : pass == AUV_SEQ_STEP ? 1024 : (int64_t)1 << 22;
     r.grid_x = want < cap ? want : cap;
     return r;

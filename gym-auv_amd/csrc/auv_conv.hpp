@@ -8,8 +8,9 @@
 // Bound by memory: one read and one write per element against 2 W + 20 operations.  A thread therefore takes a run of
 // tokens of 8 (32-bit types: 4) adjacent channels, one 16-byte access per token at any alignment, and keeps the W - 1
 // earlier tokens in registers, so that every element is read once, but for W - 1 tokens at the start of each run, which the
-// run before has just read.  bf16, width 4: 4,096 rows x 128 tokens x 128 channels 62 to 66 us forwards (268 MB, 4.2 TB/s)
-// and 101 us backwards (403 MB, 4.0 TB/s); a step of 65,536 rows 23.5 us (134 MB, 5.7 TB/s).
+// run before has just read.  bf16, width 4: 4,096 rows x 128 tokens x 128 channels 66 us forwards (268 MB, 4.1 TB/s) and 103
+// us backwards (403 MB, 3.9 TB/s; 255 registers, four spilled, two waves per SIMD); a step of 65,536 rows 24 us (134 MB, 5.6
+// TB/s).
 #pragma once
 
 #include "auv_seq.hpp"

@@ -17,8 +17,9 @@ int64_t lanes_of(int64_t channels) {
 int64_t rows_of(int64_t lanes) { return lanes < 256 ? 256 / lanes : 1; }
 
 // Workgroups of a backward pass: each leaves one record of column sums, so a workgroup takes many rows.  512 of 256
-// threads are two per CU, all that the registers hold (262,144 rows of 250 channels, forward and backward: 487 us; with
-// 768, the last of which start when the first end, 504 us).
+// threads are two per CU, all that the registers hold (262,144 rows of 250 channels, forward and backward: 450 us; with
+// 768, the last of which start when the first end, 455 us, with 256 440 us; 16,384 rows of 1,024 channels 172, 171 and 175
+// us).  256 of 1,024 threads are one per CU (8,192 rows of 4,096 channels 631 us; 128 857 us, 512 653 us).
 int64_t back_blocks(int64_t rows, int64_t channels) {
     const int64_t lanes = lanes_of(channels), want = ceil_div(rows, rows_of(lanes)), cap = lanes == 1024 ? 256 : 512;
     return want < cap ? want : cap;

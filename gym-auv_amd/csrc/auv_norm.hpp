@@ -9,7 +9,9 @@
 // Bound by memory: every element of x, y and gate is read once and of x' and h written once, against some 12
 // operations.  A row stays in registers between its two sums: TPR lanes share it, 8 adjacent elements each (16 bytes of a
 // 16-bit type), so rows of up to 32, 64, 128, 256, 512, 2,048 and 8,192 channels take 4, 8, 16, 32, 64, 256 and 1,024
-// lanes.
+// lanes.  65,536 rows of 128 channels, bf16 and 32-bit residuals: 21.5 us forwards, 5.4 TB/s.  Just above a step lanes lie
+// idle (520 channels 3.1 TB/s forwards, 512 5.5), and with 1,024 lanes the backward pass has 128 registers and spills 72 to
+// 129 (8,192 channels 3.0 TB/s forwards and backwards, 512 5.4).
 #pragma once
 
 #include "auv_seq.hpp"

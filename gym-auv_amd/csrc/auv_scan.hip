@@ -21,11 +21,11 @@ struct Chunks {
 };
 // Splits the time axis when the rows alone leave the chip short of waves: fewer than `enough`, which is one wave per SIMD
 // of the 256 CUs forwards and two backwards.  A split pays for itself only when it brings at least three chunks: every
-// element is then gone over twice.  16 states, 128 channels, 512 tokens, bf16: 128 rows backwards 288 us in four chunks,
-// 470 us whole; 512 rows forwards 187 us whole, 362 us in chunks.  (7 rows x 1,001 tokens x 90 channels, forwards and
-// backwards: 105 us with chunks for two waves per SIMD and of 32 tokens at least, 71 us for four and of 16.)
+// element is then gone over twice.  16 states, 128 channels, 512 tokens, bf16: forwards 64 rows 64 us in chunks and 84 whole,
+// 128 rows (1,024 waves) 106 and 85; forwards and backwards 128 rows 327 us with the backward pass in chunks and 486 whole,
+// 192 rows (1,536 waves) 537 and 511.
 Chunks split(int64_t L, int64_t waves, int64_t enough) {
-    constexpr int64_t kTarget = 4096;   // four waves per SIMD
+    constexpr int64_t kTarget = 4096;   // four waves per SIMD (10,075 tokens x 128 forwards: 35.6 us, 34.7 for two, 38.7 for eight)
     if (waves >= enough || waves == 0 || L == 0) return {L, 1};     // (an empty batch has no waves)
     const int64_t want = ceil_div(kTarget, waves);
     int64_t length = ceil_div(ceil_div(L, want), kSegment) * kSegment;
@@ -35,7 +35,7 @@ Chunks split(int64_t L, int64_t waves, int64_t enough) {
 
 struct Forward {
     // four states per lane instead of sixteen: four times the waves for small batches.  16 states, 128 channels, 512 tokens,
-    // bf16: 512 rows 187 us narrow, 245 us wide; 768 rows 269 and 326; 1,024 rows (two wide waves per SIMD) 327 us wide.
+    // bf16: 512 rows 179 us narrow, 249 us wide; 768 rows 272 and 321; 1,024 rows (two wide waves per SIMD) 344 and 324.
     bool narrow;
     int64_t waves;   // without chunks
     Chunks chunks;
@@ -66,8 +66,8 @@ Backward backward_plan(const auv_scan_args& p) {
     const int64_t groups = ceil_div(p.batch, r.units);
     r.chunks = split(p.length, groups * r.grid_y * waves, 2048);
     // each workgroup leaves one record of sums per row it works on side by side: as many as fill the chip, not more
-    // (4,096 rows x 64 tokens x 128 channels, 16 states, forwards and backwards: 890 us; with half of them 896, with four
-    // times as many 917)
+    // (4,096 rows x 64 tokens x 128 channels, 16 states, forwards and backwards: 825 us; with half of them 838, with twice as
+    // many 822, with four times 836)
     const int64_t cap = r.grid_y < 1024 ? 1024 / r.grid_y : 1;
     r.grid_x = groups * r.chunks.count < cap ? groups * r.chunks.count : cap;
     const int64_t NP = 4 * S;
@@ -202,8 +202,8 @@ template <class T, int S>
 int run_step(ScanArgs a, hipStream_t stream) {
     const int64_t lanes = a.D * S < kStepThreads ? a.D * S : kStepThreads, tiles = ceil_div(a.D * S, lanes);
     a.lanes = (int32_t)lanes;
-    // eight workgroups per CU, each with as many rows as it takes (65,536 rows of 64 channels, 16 states: 126 us; two per CU
-    // 153 us; a workgroup for every row 181 us)
+    // eight workgroups per CU, each with as many rows as it takes (65,536 rows of 64 channels, 16 states: 125 us; two per CU
+    // 148 us; a workgroup for every row 168 us)
     const int64_t want = ceil_div(a.B, kStepThreads / lanes), most = ceil_div(2048, tiles);
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)tiles), block(kStepThreads);
     hipLaunchKernelGGL((k_scan_step<T, S>), grid, block, 0, stream, a);

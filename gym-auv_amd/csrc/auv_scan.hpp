@@ -11,7 +11,7 @@
 // Two bounds lie close together: 4 elements of traffic per (token, channel), and per state one exponential (two issue
 // slots), two multiplications and two fused multiply-adds on the vector unit.  4,096 rows x 128 tokens x 128 channels, bf16,
 // 16 states: the traffic (638 MB) asks for 124 us, 96 slots for the states and some 45 for widths, gates, sums and their
-// loads and stores for 290 us.  It takes 296 to 328 us with the vector unit busy 90 % of the time: bound by arithmetic.
+// loads and stores for 290 us.  It takes 297 us with the vector unit at work in 92 % of the busy cycles: bound by arithmetic.
 // The product x B as a rank-1 matrix instruction (4 x 4 x 1, in 32 bits) took 444 us, C h by them as well 506 us.
 #pragma once
 
@@ -91,7 +91,7 @@ __device__ __forceinline__ float chunk_log(bool cut, float log) { return cut ? k
 template <int S>
 constexpr int lane_bits() { return S >= 16 ? 4 : S >= 8 ? 3 : S >= 4 ? 2 : S >= 2 ? 1 : 0; }
 // Tokens at a time: at least one for every lane of a channel.  Four where a lane has whole channels: eight take 233
-// registers (two waves per SIMD, 398 us for 4,096 x 128 x 128 in bf16 with 16 states), four 165 (three, 356 us).
+// registers (two waves per SIMD, 324 us for 4,096 x 128 x 128 in bf16 with 16 states), four 165 (three, 297 us).
 template <int S>
 constexpr int scan_tile() { return S > 8 ? S : S == 1 ? 4 : 8; }
 
@@ -343,10 +343,11 @@ __global__ __launch_bounds__(kJoinThreads) void k_scan_join(JoinArgs a) {
 // The element-wise parts (widths, gates and their derivatives; the stores of du, ddelta, dz) belong to the workgroup: a
 // thread takes four adjacent channels of a token, so that loads and stores are 8 or 16 bytes wide and a token's channels
 // go in one piece.  Two-byte accesses by the lanes of the sweeps, 32 bytes of a token at a time, took longer than the
-// arithmetic.  4,096 rows x 64 tokens x 128 channels, bf16, 16 states: 700 us (1,878 us in the first form, with lanes that
-// loaded for themselves and sums through shuffles) at 2,360 vector instructions per 16 tokens of 16 channels, the vector
-// unit busy 82 % of the time: bound by arithmetic.  The element-wise parts take 15 % of it, the tokens gone over twice in
-// half segments 7 %, the fetching 5 %, the sums of dB and dC 4 %.
+// arithmetic.  4,096 rows x 64 tokens x 128 channels, bf16, 16 states: 669 us (1,878 us in the first form, with lanes that
+// loaded for themselves and sums through shuffles) at 2,425 vector instructions per 16 tokens of 16 channels, the vector unit
+// at work in 94 % of the busy cycles: bound by instructions issued.  Not all of them are arithmetic: 128 registers, which two
+// workgroups per CU leave, do not hold a tile, so that 116 scalars lie in vector lanes and are moved there and back, and 21
+// vector registers (25 of 32-bit activations) in scratch memory, a good half of the 21 memory instructions per tile.
 template <int S>
 constexpr int scan_back_waves() { return S <= 4 ? 8 : 4; }
 // tokens whose states a lane holds at a time: half a segment, so that two waves more fit on a SIMD (with S = 16 the sums

@@ -95,7 +95,8 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // e^x for activations of type T.  The rounding of the product x log2(e) moves the result by |x| 2^-24 of itself: nothing
-// beside what a 16-bit x was rounded by itself, but for 32-bit ones the product is carried to twice the width,
+// beside what a 16-bit x was rounded by itself (by up to half a step, which moves e^x by |x| 2^-8 or 2^-11 of itself; so it is for
+// the scan's step width, whose x has a 32-bit bias added), but for 32-bit ones the product is carried to twice the width,
 // e^x = 2^(hi + lo), 2^lo = 1 + lo ln 2.
 template <class T>
 __device__ __forceinline__ float exp_f(float x) {

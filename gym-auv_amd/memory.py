@@ -23,7 +23,7 @@ float32; arithmetic is in 32 bits and every output is rounded once.  Calls run o
 torch's current stream of the tensors' device, never synchronise, and give the same
 bits on every call.  They can be captured into a graph.  A captured backward pass is
 refused while an eager graph of the same parameters is still alive: drop the outputs of
-earlier eager passes first.  Forward-mode derivatives and traces (torch.jit.trace,
+earlier eager passes first.  A backward pass is captured together with its forward pass.  Forward-mode derivatives and traces (torch.jit.trace,
 make_fx) are refused; torch.compile breaks its graph at these calls and runs them.
 
 `EpisodeMemory` strings them together; `cnn.PerceptionNavigationExtractor(memory=...)`
@@ -669,6 +669,8 @@ def residual_norm(x, y, post_weight=None, pre_weight=None, gate=None, scale=None
 # the operators strung together
 # ----------------------------------------------------------------------------
 class _Layer(nn.Module):
+    # What is learned per channel, the rank of the step width and the first values are those of the published method (A. Gu
+    # and T. Dao, Linear-Time Sequence Modeling with Selective State Spaces, 2023), whose arguments selective_scan takes.
     def __init__(self, channels, inner, states, width, dtype):
         super().__init__()
         self.inner, self.states, self.rank = inner, states, max(1, math.ceil(channels / 16))
