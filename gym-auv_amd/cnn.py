@@ -134,7 +134,7 @@ class PerceptionNavigationExtractor:
 
     @property
     def state(self):
-        """The memory's state of the batch, (convolution, scan) per layer; None before an episode's first call."""
+        """The memory's state of the batch, (convolution, scan) per layer; None before the first call."""
         return self._state
 
     def reset(self):

@@ -23,8 +23,9 @@ float32; arithmetic is in 32 bits and every output is rounded once.  Calls run o
 torch's current stream of the tensors' device, never synchronise, and give the same
 bits on every call.  They can be captured into a graph.  A captured backward pass is
 refused while an eager graph of the same parameters is still alive: drop the outputs of
-earlier eager passes first.  A backward pass is captured together with its forward pass.  Forward-mode derivatives and traces (torch.jit.trace,
-make_fx) are refused; torch.compile breaks its graph at these calls and runs them.
+earlier eager passes first.  A backward pass is captured together with its forward pass.
+Forward-mode derivatives and traces (torch.jit.trace, make_fx) are refused; torch.compile
+breaks its graph at these calls and runs them.
 
 `EpisodeMemory` strings them together; `cnn.PerceptionNavigationExtractor(memory=...)`
 steps one behind the scan's features.
